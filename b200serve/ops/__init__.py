@@ -12,6 +12,7 @@ from __future__ import annotations
 import math
 import os
 import threading
+from typing import NamedTuple
 
 import torch
 
@@ -1326,6 +1327,157 @@ def q4_dequant_pages(block_ids, codes, scales, out):
     ids = block_ids.long()
     out[:ids.numel()] = q4_dequantize_rows(codes[ids], scales[ids]).to(out.dtype)
     return out
+
+
+# ------------------------------------------------------------------ log probabilities
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor        # [B] fp32: log probability of the given token
+    rank: torch.Tensor           # [B] int32: tokens that rank before it (0 = the most likely)
+    entropy: torch.Tensor        # [B] fp32: entropy of the row's distribution in nats
+    top_ids: torch.Tensor        # [B, top] int32: the most likely tokens, most likely first
+    top_logprobs: torch.Tensor   # [B, top] fp32
+
+
+MAX_TOP_LOGPROBS = 32
+
+
+def _check_tokens(op, tokens, rows):
+    if tokens.dim() != 1 or tokens.shape[0] != rows or tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{op}: tokens must be int32 or int64 [{rows}], got {tokens.dtype} {tuple(tokens.shape)}")
+    return tokens.contiguous()
+
+
+def _row_logprobs(logits, tokens):
+    """(log probabilities [B, V], of the tokens [B], entropy [B], row has a distribution [B]) of fp32 logits."""
+    V = logits.shape[1]
+    logp = torch.log_softmax(logits, -1)
+    ok = ~logits.isnan().any(-1) & (logits.amax(-1).abs() < float("inf"))
+    entropy = -(logp.exp() * logp).masked_fill(logp == float("-inf"), 0.0).sum(-1)
+    known = (tokens >= 0) & (tokens < V)
+    lp = logp.gather(1, tokens.long().clamp(0, V - 1)[:, None])[:, 0]
+    nan = float("nan")
+    return logp, torch.where(known & ok, lp, nan), torch.where(ok, entropy, nan), ok
+
+
+def token_logprobs(logits, tokens, top=0) -> TokenLogprobs:
+    """Log probability and rank of ``tokens`` [B] (int32 / int64) under the rows of ``logits`` [B, V]
+    (fp32 or bf16; -inf masks an entry), with each row's entropy and its ``top`` (0..32) most
+    likely tokens. Equal logits rank by token id. Rows may be strided; V <= 1048576.
+
+    An id outside [0, V) (padding) has log probability NaN and rank -1. Where fewer than ``top``
+    entries are above -inf the rest of the alternatives are id -1 at -inf. A row without a distribution
+    (it holds a NaN or +inf, or nothing above -inf) has NaN for every number and -1 for every
+    id and rank."""
+    B, V = logits.shape
+    tokens = _check_tokens("token_logprobs", tokens, B)
+    if not 0 <= top <= MAX_TOP_LOGPROBS:
+        raise ValueError(f"token_logprobs: top must be 0..{MAX_TOP_LOGPROBS}, got {top}")
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"token_logprobs: logits must be fp32 or bf16, got {logits.dtype}")
+    if _cuda(logits, 2):
+        return TokenLogprobs(*ext().token_logprobs(logits, tokens, int(top)))
+    x = logits.float()
+    logp, lp, entropy, ok = _row_logprobs(x, tokens)
+    at = x.gather(1, tokens.long().clamp(0, V - 1)[:, None])
+    before = (x > at) | ((x == at) & (torch.arange(V)[None, :] < tokens[:, None]))
+    known = ok & (tokens >= 0) & (tokens < V)
+    rank = torch.where(known, before.sum(-1), -1).int()
+    ids = torch.full((B, top), -1, dtype=torch.int32)
+    vals = torch.full((B, top), float("-inf"))
+    n = min(top, V)
+    best = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :n]
+    vals[:, :n] = logp.gather(1, best)
+    ids[:, :n] = torch.where(vals[:, :n] == float("-inf"), -1, best).int()
+    ids[~ok], vals[~ok] = -1, float("nan")
+    return TokenLogprobs(lp, rank, entropy, ids, vals)
+
+
+def linear_logprobs(x, w, tokens, softcap=0.0):
+    """(log probability of ``tokens`` [T], entropy [T]) fp32 of the rows of x @ w^T without storing
+    the logits: x [T, H] bf16 (H a multiple of 8, rows may be strided), w the LM head [V, H] bf16, plain or
+    a PackedWeight, tokens int32 / int64. ``softcap`` > 0: logits become
+    softcap * tanh(logit / softcap). An id outside [0, V) has log probability NaN (its entropy is
+    computed); a row whose logits hold a NaN or +inf has NaN for both. A quantised LM head takes
+    linear() and token_logprobs()."""
+    T = x.shape[0]
+    tokens = _check_tokens("linear_logprobs", tokens, T)
+    packed = isinstance(w, PackedWeight)
+    if not packed and not isinstance(w, torch.Tensor):
+        raise TypeError(f"linear_logprobs: w must be a tensor or a PackedWeight, got {type(w).__name__}")
+    if x.shape[1] != w.shape[1]:
+        raise ValueError(f"linear_logprobs: x has {x.shape[1]} columns, w {w.shape[1]}")
+    if softcap < 0:
+        raise ValueError(f"linear_logprobs: softcap must not be negative, got {softcap}")
+    if _cuda(x, 2):
+        return tuple(ext().linear_logprobs(x, w.data if packed else w, w.N if packed else 0, tokens, float(softcap)))
+    logits = x.float() @ (w.unpacked() if packed else w).float().t()
+    if softcap:
+        logits = softcap * torch.tanh(logits / softcap)
+    return _row_logprobs(logits, tokens)[1:3]
+
+
+def linear_logprobs_error(reset: bool = True) -> int:
+    """First error code of linear_logprobs' bounded waits on the current device (0 = none)."""
+    return int(ext().linear_logprobs_error(reset)) if extension_loaded() else 0
+
+
+# ------------------------------------------------------------------ mixture of experts, few tokens
+MOE_LAYER_MAX_ROWS = 16
+
+
+def moe_layer(x, router, gate_up, n_gate_up, down, n_down, k, renormalize=True, first_expert=0, out=None):
+    """A whole MoE feed-forward layer for 1..16 rows (decode) in two kernels: softmax router, the ``k`` most
+    likely experts of each row (ties: the lowest id), their SwiGLU products and the weighted sum.
+
+    x [T, H] bf16 (H a multiple of 8), router [E, H] bf16 (E <= 256, k <= 16); ``gate_up`` / ``down``: this rank's
+    experts first_expert, first_expert + 1, ... packed by models.moe.pack_experts (gate and up
+    interleaved by 64 rows, ``n_gate_up`` rows per expert; ``n_down`` = H rows), or the
+    tensors it returns. ``renormalize``: the k weights sum to 1. Experts of other ranks add
+    nothing; a row that has none here comes back as zeros. Returns [T, H]."""
+    T, H = x.shape
+    if T > MOE_LAYER_MAX_ROWS:
+        raise ValueError(f"moe_layer: at most {MOE_LAYER_MAX_ROWS} rows, got {T}")
+    if n_down != H or n_gate_up % 128 or n_gate_up <= 0:
+        raise ValueError(f"moe_layer: {n_gate_up} gate/up rows (a multiple of 128) and {n_down} down rows (= H = {H})")
+    if _cuda(x, 2):
+        out = out if out is not None else torch.empty(T, H, dtype=x.dtype, device=x.device)
+        ext().moe_layer(x, router, gate_up, int(n_gate_up), down, int(n_down), int(k), bool(renormalize),
+                        int(first_expert), out)
+        return out
+    E, inner = router.shape[0], n_gate_up // 2
+    gu_rows, dn_rows = n_gate_up * ((H + 63) // 64), (H + 127) // 128 * 2 * inner
+    local = gate_up.shape[0] // gu_rows
+    if not (1 <= k <= min(16, E) and E <= 256):
+        raise ValueError(f"moe_layer: 1 to 256 experts and 1 to 16 of them per token, got {E} and {k}")
+    if local < 1 or gate_up.shape[0] != local * gu_rows or down.shape[0] != local * dn_rows:
+        raise ValueError("moe_layer: packed expert weights have the wrong shape")
+    if first_expert < 0 or first_expert + local > E:
+        raise ValueError(f"moe_layer: experts [{first_expert}, {first_expert + local}) are not among the router's {E}")
+    p = torch.softmax(x.float() @ router.float().t(), -1)
+    order = torch.sort(p, dim=-1, descending=True, stable=True).indices[:, :k]
+    wts = p.gather(1, order)
+    if renormalize:
+        wts = wts / wts.sum(-1, keepdim=True)
+    res = torch.zeros(T, H)
+    for e in range(local):
+        t_idx, j_idx = torch.nonzero(order == first_expert + e, as_tuple=True)
+        if t_idx.numel() == 0:
+            continue
+        gu = PackedWeight.from_packed(gate_up[e * gu_rows:(e + 1) * gu_rows], n_gate_up, H).unpacked().float()
+        dn = PackedWeight.from_packed(down[e * dn_rows:(e + 1) * dn_rows], H, inner).unpacked().float()
+        v = (x[t_idx].float() @ gu.t()).view(-1, inner // 64, 2, 64)
+        act = (torch.nn.functional.silu(v[:, :, 0]) * v[:, :, 1]).reshape(-1, inner) * wts[t_idx, j_idx, None]
+        res.index_add_(0, t_idx, act @ dn.t())
+    res = res.to(x.dtype)
+    if out is not None:
+        out.copy_(res)
+        return out
+    return res
+
+
+def moe_layer_error(reset: bool = True) -> int:
+    """First error code of moe_layer's bounded waits on the current device (0 = none)."""
+    return int(ext().moe_layer_error(reset)) if extension_loaded() else 0
 
 
 def gemm_error_flag(reset: bool = True) -> int:

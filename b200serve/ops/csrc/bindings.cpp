@@ -209,7 +209,20 @@ void paged_decode_attention_tq_part(torch::Tensor q_rot, torch::Tensor q_jl, tor
                                     torch::Tensor seq_lens, torch::Tensor part_acc, torch::Tensor part_ml, double scale,
                                     int64_t tps, int64_t nsplit, int64_t split_base, int64_t nsplit_total);
 
+std::vector<torch::Tensor> token_logprobs(torch::Tensor logits, torch::Tensor tokens, int64_t top);
+std::vector<torch::Tensor> linear_logprobs(torch::Tensor x, torch::Tensor w, int64_t packed_v, torch::Tensor tokens,
+                                           double softcap);
+int64_t linear_logprobs_error(bool reset);
+void moe_layer(torch::Tensor x, torch::Tensor router, torch::Tensor gate_up, int64_t n_gate_up, torch::Tensor down,
+               int64_t n_down, int64_t k, bool renormalize, int64_t first_expert, torch::Tensor out);
+int64_t moe_layer_error(bool reset);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("token_logprobs", &token_logprobs);
+  m.def("linear_logprobs", &linear_logprobs);
+  m.def("linear_logprobs_error", &linear_logprobs_error);
+  m.def("moe_layer", &moe_layer);
+  m.def("moe_layer_error", &moe_layer_error);
   m.def("paged_decode_attention_tc_part", &paged_decode_attention_tc_part);
   m.def("paged_decode_attention_tq_part", &paged_decode_attention_tq_part);
   m.def("paged_decode_combine", &paged_decode_combine);

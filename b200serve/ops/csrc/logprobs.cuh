@@ -1,0 +1,65 @@
+// Row statistics shared by the two log-probability kernels (logprobs.cu over logits in memory,
+// linear_logprobs.cu over the product of hidden states and the LM head).
+//
+// A slice of a row's logits x is summed up as m = max x, s = sum e^(x-m), t = sum e^(x-m) (x-m).
+// Slices join exactly: with M = max m_i and d_i = m_i - M,
+//   s = sum e^d_i s_i,   t = sum e^d_i (t_i + d_i s_i),
+//   log p(token) = (x_token - M) - log s,   entropy = log s - t / s.
+// Everything is fp32: every term lies in [0, 1], so a sum of V of them keeps a relative error of a
+// few 2^-24, and the differences from the maximum are exact to half an ulp.
+#pragma once
+#include "common.cuh"
+
+namespace b200 {
+
+constexpr int kMaxTop = 32;              // alternatives per row
+
+// tokens [rows] int32 or int64; ids outside [0, V) mean "no token" and come back as -1
+struct TokenIds {
+  const void* ptr;
+  int is64;
+};
+
+__device__ __forceinline__ int token_id(const TokenIds& t, long long row, int V) {
+  const long long id = t.is64 ? static_cast<const long long*>(t.ptr)[row]
+                              : (long long)static_cast<const int*>(t.ptr)[row];
+  return id >= 0 && id < V ? (int)id : -1;
+}
+
+struct RowStat {
+  float m, s, t;
+};
+
+// Adds slice (m, s, t) to `a`. m = -inf marks an empty slice (its s and t are 0).
+__device__ __forceinline__ void stat_merge(RowStat& a, const RowStat& b) {
+  const float M = fmaxf(a.m, b.m);
+  const float da = a.m - M, db = b.m - M;
+  if (a.m == -INFINITY) {
+    a = b;
+  } else if (b.m != -INFINITY) {
+    const float ea = __expf(da), eb = __expf(db);
+    a.t = ea * (a.t + da * a.s) + eb * (b.t + db * b.s);
+    a.s = ea * a.s + eb * b.s;
+    a.m = M;
+  }
+}
+
+__device__ __forceinline__ RowStat stat_warp_merge(RowStat a) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    RowStat b;
+    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+    b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
+    stat_merge(a, b);
+  }
+  return a;
+}
+
+// A row has a distribution unless it holds a NaN or +inf (s is NaN then: +inf - +inf) or nothing
+// above -inf (s stays 0).
+__device__ __forceinline__ bool stat_valid(const RowStat& a) { return a.s > 0.f && a.m < INFINITY; }
+
+__device__ __forceinline__ float stat_entropy(const RowStat& a) { return fmaxf(0.f, logf(a.s) - a.t / a.s); }
+
+}  // namespace b200
