@@ -3,15 +3,21 @@
 // the model caps them) never reach memory.
 //
 //   linear_logprobs: a persistent tcgen05 GEMM. The hidden states are the MMA's A operand (128
-//   rows = the 128 TMEM lanes), a tile of the vocabulary its B operand (tile_n <= 256 rows = TMEM
-//   columns), so a thread of the epilogue owns a row and sums up a slice's maximum and exponential
-//   sums in registers, with no exchange between threads. Per (row, tile half) 16 bytes are
-//   written instead of 4 * tile_n of logits.
+//   rows = the 128 TMEM lanes), up to 256 rows of the vocabulary its B operand (TMEM columns), so a
+//   thread of the epilogue owns a row and sums up a slice's maximum and exponential sums in
+//   registers, with no exchange between threads. Per (row, 128 columns) 16 bytes are written
+//   instead of 512 of logits.
 //   linear_logprob_rows: joins the slices of every row.
 //
-// Roles (320 threads): warp 0 TMA producer, warp 1 MMA issuer, warps 2..9 epilogue (two per TMEM
-// lane quarter, each one half of the tile's columns). The accumulator is double-buffered in TMEM, so
-// the epilogue of one tile runs under the MMAs of the next.
+// Roles (384 threads): warp 0 TMA producer, warp 1 MMA issuer, warps 4..11 epilogue (two per TMEM
+// lane quarter, 128 of the tile's columns each). The epilogue's sums need more than the 168
+// registers that 384 threads can have: the first warpgroup gives up 112 of its own to the other two.
+//
+// Sums over H. The tensor cores cut the bits that do not fit when they add to an fp32 accumulator, so
+// the error of one long sum grows with H and has a sign: 5.5e-6 of the result's norm at H = 4096, five
+// times a rounded fp32 sum's. So only 512 elements are summed up in TMEM; the epilogue adds these
+// parts to the 128 sums that each of its threads keeps in registers, rounding to nearest. The two TMEM
+// buffers alternate between parts, and the MMAs run on under the epilogue.
 //
 // Bound by the tensor cores for a prompt (2 T V H operations) and by the read of w (2 V H bytes)
 // for at most 128 rows.
@@ -25,7 +31,12 @@
 
 namespace b200 {
 
-constexpr int kLlBM = 128, kLlBN = 256, kLlBK = 64, kLlStages = 4, kLlThreads = 320;
+constexpr int kLlBM = 128, kLlBN = 256, kLlBK = 64, kLlStages = 4, kLlThreads = 384;
+// registers per thread: at launch, of the producer's and the MMA issuer's warpgroup, of the epilogue's two
+constexpr int kLlRegs = 168, kLlRegsLow = 56, kLlRegsHigh = 224;
+static_assert(128 * kLlRegsLow + 256 * kLlRegsHigh == kLlThreads * kLlRegs, "the split must use what the block has");
+constexpr int kLlCols = kLlBN / 2;       // columns of an epilogue thread = of a slice
+constexpr int kLlPart = 8;               // 64-element blocks of H summed up in TMEM
 constexpr int kLlA = kLlBM * kLlBK * 2, kLlW = kLlBN * kLlBK * 2, kLlStage = kLlA + kLlW;
 constexpr size_t kLlSmem = 1024 + (size_t)kLlStages * kLlStage + 256;
 constexpr float kLlMasked = -1e30f;      // columns past the vocabulary: e^(x - m) is 0, products stay finite
@@ -33,24 +44,42 @@ constexpr int64_t kLlRows = 8192;        // rows per pass: bounds the partial re
 
 static __device__ int g_ll_err;          // first error code of the bounded waits, one word per device
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
+// Work units: every row tile with `main_tiles` vocabulary tiles of 256 columns, in whole waves over
+// the SMs, then with `tail_tiles` of tail_n columns for the rest, so that the last wave is short.
 struct LlArgs {
-  int T, V, kb_total, m_tiles, v_tiles, tile_n, box_rows;
+  int T, V, kb_total, m_tiles, main_tiles, tail_tiles, tail_n;
   int packed;                            // w: tile-packed [n_tile][k_block][128][64], else plain [V, H]
   float softcap;
   TokenIds tokens;
-  float4* part;                          // [2 v_tiles][T] (m, s, t, the token's logit where the slice has it)
+  int slices;                            // of 128 columns in the main part, of tail_n after it
+  float4* part;                          // [slices][T] (m, s, t, the token's logit where the slice has it)
 };
+
+struct LlUnit {
+  int m0, v0, n, slice;                  // first row, first column, columns, first slice
+};
+
+__device__ __forceinline__ LlUnit ll_unit(const LlArgs& a, int u) {
+  LlUnit x;
+  const int v = u / a.m_tiles;           // the row tiles of one vocabulary tile follow one another
+  x.m0 = (u - v * a.m_tiles) * kLlBM;
+  if (v < a.main_tiles) {
+    x.v0 = v * kLlBN;
+    x.n = kLlBN;
+    x.slice = 2 * v;
+  } else {
+    const int per = a.tail_n > kLlCols ? 2 : 1;
+    x.v0 = a.main_tiles * kLlBN + (v - a.main_tiles) * a.tail_n;
+    x.n = a.tail_n;
+    x.slice = 2 * a.main_tiles + (v - a.main_tiles) * per;
+  }
+  return x;
+}
 
 template <bool CAP>
 __global__ void __launch_bounds__(kLlThreads, 1)
     linear_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
-                           const LlArgs a) {
+                           const __grid_constant__ CUtensorMap tm_tail, const LlArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_x = smem;
@@ -63,7 +92,7 @@ __global__ void __launch_bounds__(kLlThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int units = a.m_tiles * a.v_tiles;
+  const int units = a.m_tiles * (a.main_tiles + a.tail_tiles);
   int* err = &g_ll_err;
 
   if (threadIdx.x == 0) {
@@ -88,52 +117,55 @@ __global__ void __launch_bounds__(kLlThreads, 1)
   pdl_wait();
   pdl_trigger();
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLlRegsLow));
+    if (warp == 0 && lane == 0) {
       // ---------------- TMA producer ----------------
       const uint64_t pol_w = tc::policy_evict_first(), pol_x = tc::policy_evict_last();
-      const uint32_t bytes = kLlA + a.tile_n * kLlBK * 2;
       int stage = 0;
       uint32_t phase = 0;
       for (int u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {
-        const int m0 = (u % a.m_tiles) * kLlBM, v0 = (u / a.m_tiles) * a.tile_n;
+        const LlUnit x = ll_unit(a, u);
+        const CUtensorMap* map = x.n == kLlBN ? &tm_w : &tm_tail;
+        const int box = min(x.n, 128);                     // rows per box; never across a 128-row weight tile
         for (int kb = 0; kb < a.kb_total; ++kb) {
           if (!tc::mbar_wait_bounded(&empty[stage], phase ^ 1, abort_flag, err, 11)) break;
-          tc::mbar_arrive_expect_tx(&full[stage], bytes);
-          tc::tma_load_2d(s_x + stage * kLlA, &tm_x, &full[stage], kb * kLlBK, m0, pol_x);
-          for (int r = 0; r < a.tile_n; r += a.box_rows) {
-            const int v = v0 + r;
+          tc::mbar_arrive_expect_tx(&full[stage], kLlA + x.n * kLlBK * 2);
+          tc::tma_load_2d(s_x + stage * kLlA, &tm_x, &full[stage], kb * kLlBK, x.m0, pol_x);
+          for (int r = 0; r < x.n; r += box) {
+            const int v = x.v0 + r;
             const int y = a.packed ? ((v >> 7) * a.kb_total + kb) * 128 + (v & 127) : v;
-            tc::tma_load_2d(s_w + stage * kLlW + r * 128, &tm_w, &full[stage], a.packed ? 0 : kb * kLlBK, y, pol_w);
+            tc::tma_load_2d(s_w + stage * kLlW + r * 128, map, &full[stage], a.packed ? 0 : kb * kLlBK, y, pol_w);
           }
           if (++stage == kLlStages) { stage = 0; phase ^= 1; }
         }
       }
     }
-    __syncwarp();
-  } else if (warp == 1) {
-    if (lane == 0) {
+    if (warp == 1 && lane == 0) {
       // ---------------- MMA issuer ----------------
-      const uint32_t idesc = tc::idesc_bf16_f32(kLlBM, a.tile_n);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       for (int u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {
-        if (!tc::mbar_wait_bounded(&tempty[acc], acc_phase ^ 1, abort_flag, err, 12)) break;
-        tc::tc_fence_after();
-        const uint32_t d = tmem_base + acc * kLlBN;
-        for (int kb = 0; kb < a.kb_total; ++kb) {
-          if (!tc::mbar_wait_bounded(&full[stage], phase, abort_flag, err, 13)) break;
+        const uint32_t idesc = tc::idesc_bf16_f32(kLlBM, ll_unit(a, u).n);
+        for (int k0 = 0; k0 < a.kb_total; k0 += kLlPart) {
+          if (!tc::mbar_wait_bounded(&tempty[acc], acc_phase ^ 1, abort_flag, err, 12)) break;
           tc::tc_fence_after();
-          const uint64_t da = tc::sw128_kmajor_desc(tc::smem_u32(s_x + stage * kLlA));
-          const uint64_t db = tc::sw128_kmajor_desc(tc::smem_u32(s_w + stage * kLlW));
+          const uint32_t d = tmem_base + acc * kLlBN;
+          const int kn = min(kLlPart, a.kb_total - k0);
+          for (int kb = 0; kb < kn; ++kb) {
+            if (!tc::mbar_wait_bounded(&full[stage], phase, abort_flag, err, 13)) break;
+            tc::tc_fence_after();
+            const uint64_t da = tc::sw128_kmajor_desc(tc::smem_u32(s_x + stage * kLlA));
+            const uint64_t db = tc::sw128_kmajor_desc(tc::smem_u32(s_w + stage * kLlW));
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) tc::mma_bf16(d, da + 2 * kk, db + 2 * kk, idesc, (kb | kk) ? 1u : 0u);
-          tc::mma_commit(&empty[stage]);
-          if (++stage == kLlStages) { stage = 0; phase ^= 1; }
+            for (int kk = 0; kk < 4; ++kk) tc::mma_bf16(d, da + 2 * kk, db + 2 * kk, idesc, (kb | kk) ? 1u : 0u);
+            tc::mma_commit(&empty[stage]);
+            if (++stage == kLlStages) { stage = 0; phase ^= 1; }
+          }
+          tc::mma_commit(&tfull[acc]);
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1;
         }
-        tc::mma_commit(&tfull[acc]);
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1;
       }
       // no tcgen05.mma may still be running when TMEM is released below
       tc::mma_commit(mma_done);
@@ -142,65 +174,71 @@ __global__ void __launch_bounds__(kLlThreads, 1)
     }
     __syncwarp();
   } else {
-    // ---------------- epilogue (warps 2..9) ----------------
-    const int quad = warp & 3, half = (warp - 2) >> 2;
-    const int c_lo = half ? (a.tile_n / 32) * 16 : 0;      // columns of this half, multiples of 16
-    const int c_hi = half ? a.tile_n : (a.tile_n / 32) * 16;
+    // ---------------- epilogue (warps 4..11) ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLlRegsHigh));
+    const int quad = warp & 3, half = (warp - 4) >> 2;
     const float L2E = 1.4426950408889634f;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {
-      const int row = (u % a.m_tiles) * kLlBM + quad * 32 + lane;
-      const int v_tile = u / a.m_tiles, v0 = v_tile * a.tile_n;
-      const int tok = row < a.T ? token_id(a.tokens, row, a.V) : -1;
-      if (!tc::mbar_wait_bounded(&tfull[acc], acc_phase, abort_flag, err, 14)) break;
-      tc::tc_fence_after();
-      const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * kLlBN;
-      RowStat r{kLlMasked, 0.f, 0.f};
-      float xt = 0.f;
-      for (int c0 = c_lo; c0 < c_hi; c0 += 16) {
-        float v[16];
-        tc::tmem_ld16(t_row + c0, v);
-        if constexpr (CAP) {
+      const LlUnit x = ll_unit(a, u);
+      const int row = x.m0 + quad * 32 + lane;
+      const int cols = min(x.n - half * kLlCols, kLlCols); // <= 0: this half of a narrow tile has none
+      float v[kLlCols];
+      bool live = true;
+      for (int k0 = 0; k0 < a.kb_total; k0 += kLlPart) {
+        live = tc::mbar_wait_bounded(&tfull[acc], acc_phase, abort_flag, err, 14);
+        if (!live) break;
+        tc::tc_fence_after();
+        const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * kLlBN + half * kLlCols;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = a.softcap * tanhf(v[j] / a.softcap);
+        for (int c = 0; c < kLlCols; c += 16) {
+          float r[16];                                     // columns past a narrow tile: masked below
+          tc::tmem_ld16(t_row + c, r);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[c + j] = k0 == 0 ? r[j] : v[c + j] + r[j];
         }
-        if (v0 + c0 + 16 > a.V) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (v0 + c0 + j >= a.V) v[j] = kLlMasked;
-        }
-        const int at = tok - (v0 + c0);
-        if ((unsigned)at < 16u) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) xt = j == at ? v[j] : xt;
-        }
-        float m = r.m;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) m = fmaxf(m, v[j]);
-        const float dm = r.m - m, sc = ex2(dm * L2E);
-        float s = 0.f, t = 0.f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float d = v[j] - m;
-          const float e = ex2(d * L2E);
-          s += e;
-          t = fmaf(e, fmaxf(d, kLlMasked), t);      // a logit of -inf: 0 * -1e30
-        }
-        r.t = fmaf(sc, fmaf(dm, r.s, r.t), t);
-        r.s = fmaf(sc, r.s, s);
-        r.m = m;
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&tempty[acc]);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
       }
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&tempty[acc]);
-      // a half without a column of the vocabulary, or without columns at all, holds nothing
-      const bool some = c_lo < c_hi && v0 + c_lo < a.V;
+      if (!live) break;
+      if (cols <= 0) continue;
+      const int c0 = x.v0 + half * kLlCols;                // first column; `in` of them are of the vocabulary
+      const int in = min(cols, a.V - c0);
+      if constexpr (CAP) {
+#pragma unroll
+        for (int j = 0; j < kLlCols; ++j) v[j] = a.softcap * tanhf(v[j] / a.softcap);
+      }
+      if (in < kLlCols) {
+#pragma unroll
+        for (int j = 0; j < kLlCols; ++j)
+          if (j >= in) v[j] = kLlMasked;
+      }
+      float xt = 0.f;
+      const int at = row < a.T ? token_id(a.tokens, row, a.V) - c0 : -1;
+      if ((unsigned)at < (unsigned)in) {
+#pragma unroll
+        for (int j = 0; j < kLlCols; ++j) xt = j == at ? v[j] : xt;
+      }
+      float m[4] = {kLlMasked, kLlMasked, kLlMasked, kLlMasked};
+#pragma unroll
+      for (int j = 0; j < kLlCols; ++j) m[j & 3] = fmaxf(m[j & 3], v[j]);
+      m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      float s[4] = {0.f, 0.f, 0.f, 0.f}, t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < kLlCols; ++j) {
+        const float d = v[j] - m[0];
+        const float e = ex2(d * L2E);
+        s[j & 3] += e;
+        t[j & 3] = fmaf(e, fmaxf(d, kLlMasked), t[j & 3]); // a logit of -inf: 0 * -1e30
+      }
+      const float ss = (s[0] + s[1]) + (s[2] + s[3]), tt = (t[0] + t[1]) + (t[2] + t[3]);
       if (row < a.T)
-        a.part[(size_t)(2 * v_tile + half) * a.T + row] =
-            some ? make_float4(r.s == r.s ? r.m : INFINITY, r.s, r.t, xt) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1;
+        a.part[(size_t)(x.slice + half) * a.T + row] =
+            in > 0 ? make_float4(ss == ss ? m[0] : INFINITY, ss, tt, xt) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
     }
   }
   tc::tc_fence_before();
@@ -217,7 +255,7 @@ __global__ void __launch_bounds__(kLlThreads, 1)
   }
 }
 
-// 256 threads per CTA on R rows (32: lane = row; 1: the CTA's threads share a row's slices)
+// 256 threads per CTA on R rows, neighbouring threads on neighbouring rows
 constexpr int kLlRowThreads = 256;
 template <int R>
 __global__ void __launch_bounds__(kLlRowThreads) linear_logprob_rows_kernel(const LlArgs a, float* __restrict__ logprob,
@@ -228,11 +266,10 @@ __global__ void __launch_bounds__(kLlRowThreads) linear_logprob_rows_kernel(cons
   pdl_trigger();
   const int r = threadIdx.x % R, g = threadIdx.x / R;
   const int row = blockIdx.x * R + r;
-  const int S = 2 * a.v_tiles;
   RowStat acc{-INFINITY, 0.f, 0.f};
   if (row < a.T) {
-#pragma unroll 4
-    for (int i = g; i < S; i += G) {
+#pragma unroll 8
+    for (int i = g; i < a.slices; i += G) {
       const float4 p = __ldcg(a.part + (size_t)i * a.T + row);
       stat_merge(acc, RowStat{p.x, p.y, p.z});
     }
@@ -253,9 +290,9 @@ __global__ void __launch_bounds__(kLlRowThreads) linear_logprob_rows_kernel(cons
   const int tok = token_id(a.tokens, row, a.V);
   float xt = NAN;
   if (tok >= 0) {
-    const int v_tile = tok / a.tile_n;
-    const int half = tok - v_tile * a.tile_n >= (a.tile_n / 32) * 16;
-    xt = __ldcg(&a.part[(size_t)(2 * v_tile + half) * a.T + row].w);
+    const int tail = tok - a.main_tiles * kLlBN;         // its column in the narrow tiles
+    const int slice = tail < 0 ? tok / kLlCols : 2 * a.main_tiles + tail / min(a.tail_n, kLlCols);
+    xt = __ldcg(&a.part[(size_t)slice * a.T + row].w);
   }
   logprob[row] = ok ? (xt - acc.m) - logf(acc.s) : NAN;
   entropy[row] = ok ? stat_entropy(acc) : NAN;
@@ -295,43 +332,49 @@ std::vector<torch::Tensor> linear_logprobs(torch::Tensor x, torch::Tensor w, int
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   auto stream = at::cuda::getCurrentCUDAStream();
   auto kernel = softcap > 0.0 ? linear_logprobs_kernel<true> : linear_logprobs_kernel<false>;
+  cudaFuncAttributes attr;
+  B200_REQUIRE_CUDA(cudaFuncGetAttributes(&attr, kernel));
+  B200_REQUIRE(attr.numRegs == kLlRegs, "linear_logprobs: the register split does not fit this build");
   B200_REQUIRE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLlSmem));
   torch::Tensor part;
   for (int64_t t0 = 0; t0 < T; t0 += kLlRows) {
     LlArgs a{};
     a.T = (int)std::min(kLlRows, T - t0); a.V = (int)V; a.kb_total = kb; a.packed = packed;
     a.m_tiles = (a.T + kLlBM - 1) / kLlBM;
-    // columns per tile: of the multiples of 16 from 128 to 256 the one whose busiest CTA has the
-    // fewest columns to compute (ties: the widest, which reads x least often)
+    // whole waves of 256-column tiles; the columns that are left go to tiles of the width whose
+    // waves take the least time (16 more columns stand for what a tile costs at any width)
+    const int64_t all = (V + kLlBN - 1) / kLlBN, waves = a.m_tiles * all / sms;
+    a.main_tiles = (int)std::min(V / kLlBN, waves * sms / a.m_tiles);
+    const int64_t rest = V - (int64_t)a.main_tiles * kLlBN;
     int64_t best = INT64_MAX;
-    for (int n = kLlBN; n >= 128; n -= 16) {
-      const int64_t units = (int64_t)a.m_tiles * ((V + n - 1) / n);
-      const int64_t cost = (units + sms - 1) / sms * n;
-      if (cost < best) { best = cost; a.tile_n = n; }
+    a.tail_n = kLlBN;
+    for (int n = kLlBN; n >= 16 && rest > 0; n /= 2) {
+      const int64_t cost = (a.m_tiles * ((rest + n - 1) / n) + sms - 1) / sms * (n + 16);
+      if (cost < best) { best = cost; a.tail_n = n; }
     }
-    a.v_tiles = (int)((V + a.tile_n - 1) / a.tile_n);
-    // rows per box: a divisor of the tile that keeps a box inside one 128-row weight tile
-    a.box_rows = std::min(a.tile_n & -a.tile_n, 128);
+    a.tail_tiles = (int)((rest + a.tail_n - 1) / a.tail_n);
+    a.slices = 2 * a.main_tiles + a.tail_tiles * (a.tail_n > kLlCols ? 2 : 1);
     a.softcap = (float)softcap;
     const bool is64 = tokens.scalar_type() == at::kLong;
     a.tokens = TokenIds{static_cast<const char*>(tokens.data_ptr()) + t0 * (is64 ? 8 : 4), is64};
-    const int64_t need = 2 * (int64_t)a.v_tiles * a.T * 4;
+    const int64_t need = (int64_t)a.slices * a.T * 4;
     if (!part.defined() || part.numel() < need) part = torch::empty({need}, logprob.options());
     a.part = reinterpret_cast<float4*>(part.data_ptr());
     const void* xp = static_cast<const __nv_bfloat16*>(x.data_ptr()) + t0 * ldx;
     const uint64_t xd[2] = {(uint64_t)H, (uint64_t)a.T}, xs[1] = {(uint64_t)ldx * 2};
     const uint32_t xb[2] = {64, kLlBM};
     const uint64_t wd[2] = {packed ? 64ull : (uint64_t)H, (uint64_t)w.size(0)}, ws[1] = {(packed ? 64 : H) * 2ull};
-    const uint32_t wb[2] = {64, (uint32_t)a.box_rows};
-    const CUtensorMap tx = tma_bf16(xp, 2, xd, xs, xb), tw = tma_bf16(w.data_ptr(), 2, wd, ws, wb);
-    const int64_t units = (int64_t)a.m_tiles * a.v_tiles;
+    const uint32_t wb[2] = {64, 128}, tb[2] = {64, (uint32_t)std::min(a.tail_n, 128)};
+    const CUtensorMap tx = tma_bf16(xp, 2, xd, xs, xb), tw = tma_bf16(w.data_ptr(), 2, wd, ws, wb),
+                      tt = tma_bf16(w.data_ptr(), 2, wd, ws, tb);
+    const int64_t units = (int64_t)a.m_tiles * (a.main_tiles + a.tail_tiles);
     const unsigned grid = (unsigned)std::min<int64_t>(units, sms);
-    launch_pdl(kernel, dim3(grid), dim3(kLlThreads), kLlSmem, stream, tx, tw, a);
+    launch_pdl(kernel, dim3(grid), dim3(kLlThreads), kLlSmem, stream, tx, tw, tt, a);
     float* lp = logprob.data_ptr<float>() + t0;
     float* en = entropy.data_ptr<float>() + t0;
-    if (a.T >= 64)
-      launch_pdl(linear_logprob_rows_kernel<32>, dim3((unsigned)((a.T + 31) / 32)), dim3(kLlRowThreads), 0, stream, a,
-                 lp, en);
+    if (a.T >= 8)
+      launch_pdl(linear_logprob_rows_kernel<8>, dim3((unsigned)((a.T + 7) / 8)), dim3(kLlRowThreads), 0, stream, a, lp,
+                 en);
     else
       launch_pdl(linear_logprob_rows_kernel<1>, dim3((unsigned)a.T), dim3(kLlRowThreads), 0, stream, a, lp, en);
   }

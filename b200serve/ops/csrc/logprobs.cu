@@ -7,13 +7,15 @@
 //     work on one read. Bound by HBM (4 or 2 bytes a logit) once there are rows for every SM.
 //   * logprob_rows: one CTA per row joins the slices' statistics and merges their sorted lists.
 //
-// Selection. Logit and id make one 64-bit key (order-preserving bits of the value, then the
-// complement of the id), so keys are unique and "ties: the lowest id" is the key order. The `top`-th
-// largest of the 256 per-thread maxima is at most the `top`-th largest key of the slice; one warp
-// finds a value with at least `top` and at most top + 12 maxima above it by descending the key
-// bits. Only those threads push keys, at most 32 each, into a list that is ranked by counting. The
-// bound on the list holds for any data (all logits equal, sorted rows), so no case needs a
-// second way.
+// Selection. The `top`-th largest of the 256 per-thread maxima is at most the `top`-th largest logit
+// of the slice. One warp finds a value with at least `top` and at most top + 12 maxima at or above
+// it by descending the bits of the (order-preserving) values; only those threads look at their 32
+// or 64 logits again and push what reaches the value into a list, which is ranked by counting. The
+// rank goes by a 64-bit key (value bits, then the complement of the id), so keys are unique and
+// "ties: the lowest id" is the key order. Where too many maxima are equal for any value to do,
+// the same search runs over the keys of the maxima instead. Either way the list is bounded by
+// (top + 12) threads' logits, for any data. The row kernel selects among the slices' lists
+// the same way, from the lists' heads.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -48,15 +50,37 @@ struct LpArgs {
   unsigned long long* keys;              // [B][S][top] descending, 0 = none
 };
 
+// The largest value whose bits, from `bit` down to 0, can be set with at least `top` of the warp's N * 32
+// keys at or above it; stops early at top + kLpSlack. Returns the number of keys at or above it.
+template <typename K, int N>
+__device__ __forceinline__ int key_threshold(const K (&k)[N], int top, int bit, K& thr) {
+  int have = N * 32;
+  for (; bit >= 0; --bit) {
+    const K c = thr | (K(1) << bit);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) n += k[i] >= c;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (n >= top) {
+      thr = c;
+      have = n;
+      if (n <= top + kLpSlack) break;
+    }
+  }
+  return have;
+}
+
 // T = float or __nv_bfloat16; U 16-byte pieces per thread
 template <typename T, int U>
-__global__ void __launch_bounds__(kLpThreads) logprob_slices_kernel(const LpArgs a) {
-  constexpr int VEC = 16 / (int)sizeof(T), NV = U * VEC, SLICE = kLpThreads * NV;
+__global__ void __launch_bounds__(kLpThreads, U == 8 && sizeof(T) == 2 ? 2 : 4) logprob_slices_kernel(const LpArgs a) {
+  constexpr int VEC = 16 / (int)sizeof(T), NV = U * VEC, SLICE = kLpThreads * NV, WARPS = kLpThreads / 32;
   constexpr int CAP = (kMaxTop + kLpSlack) * NV;
-  __shared__ float red[kLpThreads / 32][4];
-  __shared__ unsigned long long tmax[kLpThreads];
+  __shared__ float red[WARPS][4];
+  __shared__ uint32_t tmax[kLpThreads];
+  __shared__ unsigned long long tkey[kLpThreads];
   __shared__ unsigned long long list[CAP];
-  __shared__ unsigned long long thr_s;
+  __shared__ float thr_s;
+  __shared__ unsigned long long thr_key_s;
   __shared__ int count_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long row = blockIdx.x / a.S;
@@ -66,14 +90,15 @@ __global__ void __launch_bounds__(kLpThreads) logprob_slices_kernel(const LpArgs
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
   // 16-byte pieces are counted from the last aligned address at or before the row
   const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const int base = slice * SLICE - shift;              // id of this slice's first element (may be < 0)
+  const int base = slice * SLICE - shift + tid * VEC;  // id of this thread's first element (may be < 0)
+  auto id_of = [&](int i) { return base + (i / VEC) * kLpThreads * VEC + i % VEC; };
   const int tok = token_id(a.tokens, row, a.V);
   const float xt = tok >= 0 ? (float)x[tok] : INFINITY;
 
   float v[NV];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int id0 = base + (u * kLpThreads + tid) * VEC;
+    const int id0 = id_of(u * VEC);
     if (id0 >= 0 && id0 + VEC <= a.V) {
       const uint4 w = *reinterpret_cast<const uint4*>(x + id0);
       if constexpr (VEC == 4) {
@@ -96,95 +121,106 @@ __global__ void __launch_bounds__(kLpThreads) logprob_slices_kernel(const LpArgs
 #pragma unroll
   for (int i = 0; i < NV; ++i) tm = fmaxf(tm, v[i]);
   const float wm = warp_max(tm);
-  if (lane == 0) red[warp][0] = wm;
-  // the thread's largest key: its maximum at the lowest id that holds it
+  if (lane == 0) red[warp][3] = wm;
   if (a.top > 0) {
-    unsigned long long k = 0;
-    if (tm > -INFINITY) {
-      int at = 0;
-#pragma unroll
-      for (int i = NV - 1; i >= 0; --i)
-        if (v[i] == tm) at = (i / VEC) * kLpThreads * VEC + i % VEC;
-      k = logit_key(tm, base + tid * VEC + at);
-    }
-    tmax[tid] = k;
+    tmax[tid] = logit_bits(tm);
     if (tid == 0) count_s = 0;
   }
   __syncthreads();
-  float m = red[0][0];
+  float m = red[0][3];
 #pragma unroll
-  for (int i = 1; i < kLpThreads / 32; ++i) m = fmaxf(m, red[i][0]);
+  for (int i = 1; i < WARPS; ++i) m = fmaxf(m, red[i][3]);
+
+  // ---- threshold (the other warps go on with the sums)
+  if (a.top > 0 && warp == WARPS - 1) {
+    uint32_t k[WARPS], any = 0, all = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+      k[i] = tmax[i * 32 + lane];
+      any |= k[i];
+      all &= k[i];
+    }
+    any = __reduce_or_sync(0xffffffffu, any);
+    all = __reduce_and_sync(0xffffffffu, all);
+    // the bits above the highest one in which the maxima differ are common to all of them
+    const int bit = 31 - __clz((any & ~all) | 1u);
+    uint32_t thr = bit == 31 ? 0u : all >> (bit + 1) << (bit + 1);
+    const int n = key_threshold<uint32_t>(k, a.top, bit, thr);
+    // 0: fewer than `top` threads hold a logit above -inf; all logits are candidates
+    if (lane == 0) thr_s = thr == 0u ? -3.402823466e38f : n <= a.top + kLpSlack ? logit_of_bits(thr) : NAN;
+  }
 
   // ---- sums and the count of logits that rank before the token
   const float mm = m == -INFINITY ? 0.f : m;
   float s = 0.f, t = 0.f;
   int cnt = 0;
+  bool equal = false;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int id = base + ((i / VEC) * kLpThreads + tid) * VEC + i % VEC;
     const float d = v[i] - mm;
-    const float e = __expf(d);
+    const float e = ex2(d * 1.4426950408889634f);
     s += e;
-    t += e * fmaxf(d, -1e30f);                         // a masked logit: e = 0, d = -inf
+    t = fmaf(e, fmaxf(d, -1e30f), t);                  // a masked logit: e = 0, d = -inf
     cnt += v[i] > xt;
-    // padding outside the row is -inf too: only ids of the row count
-    if (v[i] == xt && id >= 0 && id < tok) ++cnt;
+    equal |= v[i] == xt;
+  }
+  if (equal) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)                       // padding outside the row is -inf too: only ids of the row count
+      cnt += v[i] == xt && id_of(i) >= 0 && id_of(i) < tok;
   }
   s = warp_sum(s);
   t = warp_sum(t);
   cnt = __reduce_add_sync(0xffffffffu, cnt);
-  __syncthreads();                                     // red[][0] was read above
   if (lane == 0) { red[warp][0] = s; red[warp][1] = t; red[warp][2] = __int_as_float(cnt); }
-
-  // ---- threshold: at least `top` per-thread maxima lie at or above it
-  if (a.top > 0 && warp == 0) {
-    unsigned long long k[kLpThreads / 32];
-    uint32_t hi_or = 0, hi_and = 0xffffffffu;
-#pragma unroll
-    for (int i = 0; i < kLpThreads / 32; ++i) {
-      k[i] = tmax[i * 32 + lane];
-      hi_or |= (uint32_t)(k[i] >> 32);
-      hi_and &= (uint32_t)(k[i] >> 32);
-    }
-    hi_or = __reduce_or_sync(0xffffffffu, hi_or);
-    hi_and = __reduce_and_sync(0xffffffffu, hi_and);
-    // bits above the highest differing one are common to all keys
-    const uint32_t diff = hi_or & ~hi_and;
-    int bit = diff ? 63 - __clz(diff) : 31;
-    unsigned long long thr = bit == 63 ? 0ull : (((unsigned long long)hi_and << 32) >> (bit + 1)) << (bit + 1);
-    for (; bit >= 0; --bit) {
-      const unsigned long long c = thr | (1ull << bit);
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < kLpThreads / 32; ++i) n += k[i] >= c;
-      n = __reduce_add_sync(0xffffffffu, n);
-      if (n >= a.top) {
-        thr = c;
-        if (n <= a.top + kLpSlack) break;
-      }
-    }
-    if (lane == 0) thr_s = thr ? thr : 1ull;           // fewer than `top` threads hold a key: all keys
-  }
   __syncthreads();
   if (tid == 0) {
     float bs = 0.f, bt = 0.f;
     int bc = 0;
 #pragma unroll
-    for (int i = 0; i < kLpThreads / 32; ++i) { bs += red[i][0]; bt += red[i][1]; bc += __float_as_int(red[i][2]); }
+    for (int i = 0; i < WARPS; ++i) { bs += red[i][0]; bt += red[i][1]; bc += __float_as_int(red[i][2]); }
     // a NaN (of the data, or +inf - +inf) marks the row through m = +inf
     a.part[row * a.S + slice] = make_float4(bs == bs ? m : INFINITY, bs, bt, __int_as_float(bc));
   }
   if (a.top == 0) return;
 
-  // ---- candidates
-  const unsigned long long thr = thr_s;
-  if (tmax[tid] >= thr) {
+  // ---- candidates (the order of the list does not matter)
+  const float thr = thr_s;
+  if (thr == thr) {
+    if (tm >= thr) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const unsigned long long k = logit_key(v[i], base + ((i / VEC) * kLpThreads + tid) * VEC + i % VEC);
-      if (k >= thr) {
-        const int p = atomicAdd(&count_s, 1);          // the order of the list does not matter
-        if (p < CAP) list[p] = k;
+      for (int i = 0; i < NV; ++i)
+        if (v[i] >= thr) {
+          const int p = atomicAdd(&count_s, 1);
+          if (p < CAP) list[p] = logit_key(v[i], id_of(i));
+        }
+    }
+  } else {
+    // too many equal maxima: a thread's largest key is its maximum at the lowest id that holds it
+    int at = 0;
+#pragma unroll
+    for (int i = NV - 1; i >= 0; --i)
+      if (v[i] == tm) at = id_of(i);
+    const unsigned long long mine = logit_key(tm, at);
+    tkey[tid] = mine;
+    __syncthreads();
+    if (warp == 0) {
+      unsigned long long k[WARPS], key = 0;
+#pragma unroll
+      for (int i = 0; i < WARPS; ++i) k[i] = tkey[i * 32 + lane];
+      key_threshold<unsigned long long>(k, a.top, 63, key);
+      if (lane == 0) thr_key_s = key;
+    }
+    __syncthreads();
+    const unsigned long long key = thr_key_s;
+    if (mine >= key) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const unsigned long long k = logit_key(v[i], id_of(i));
+        if (k >= key) {
+          const int p = atomicAdd(&count_s, 1);
+          if (p < CAP) list[p] = k;
+        }
       }
     }
   }
@@ -208,58 +244,75 @@ struct LpOut {
   float* top_lp;                         // [B][top]
 };
 
-// One CTA of 128 threads per row. Warp 0 joins the statistics; the slices' sorted lists are
-// staged in shared memory, lane l walks the heads of lists l, l + 32, ... and every round takes
-// the largest head of the warp.
-constexpr int kLpRowThreads = 128;
+// One CTA of 256 threads per row. Warp 0 joins the statistics. With S lists of `top` keys, sorted, the
+// r-th largest of the d-th entries, d = max(1, ceil(top / S)) and r = ceil(top / d), has at least
+// r d >= top keys at or above it: what reaches it is collected and ranked by counting.
+constexpr int kLpRowThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kLpRowThreads) logprob_rows_kernel(const LpArgs a, const LpOut o) {
-  extern __shared__ unsigned long long lists[];        // [S][top], then one int per list
-  int* head = reinterpret_cast<int*>(lists + (size_t)a.S * a.top);
-  const int tid = threadIdx.x, lane = tid & 31;
+  extern __shared__ unsigned long long lists[];        // [S][top], then the candidates [S][top]
+  __shared__ unsigned long long thr_s;
+  __shared__ int count_s;
+  __shared__ float max_s, log_s_s;
+  const int tid = threadIdx.x, lane = tid & 31, total = a.S * a.top;
   const long long row = blockIdx.x;
+  if (tid == 0) { thr_s = 0ull; count_s = 0; }
   pdl_wait();
   pdl_trigger();
-  const unsigned long long* src = a.keys + row * a.S * a.top;
-  for (int i = tid; i < a.S * a.top; i += kLpRowThreads) lists[i] = __ldcg(src + i);
-  if (a.top > 0)
-    for (int i = tid; i < a.S; i += kLpRowThreads) head[i] = 0;
-  __syncthreads();
-  if (tid >= 32) return;
-  RowStat r{-INFINITY, 0.f, 0.f};
-  int cnt = 0;
-  for (int i = lane; i < a.S; i += 32) {
-    const float4 p = __ldcg(a.part + row * a.S + i);
-    stat_merge(r, RowStat{p.x, p.y, p.z});
-    cnt += __float_as_int(p.w);
-  }
-  r = stat_warp_merge(r);
-  cnt = __reduce_add_sync(0xffffffffu, cnt);
-  const bool ok = stat_valid(r);
-  const float log_s = ok ? logf(r.s) : NAN;
-  if (lane == 0) {
-    const int tok = token_id(a.tokens, row, a.V);
-    const float xt = tok >= 0 ? (float)(static_cast<const T*>(a.logits) + row * a.ld)[tok] : NAN;
-    o.logprob[row] = (xt - r.m) - log_s;
-    o.rank[row] = ok && tok >= 0 ? cnt : -1;
-    o.entropy[row] = ok ? stat_entropy(r) : NAN;
-  }
-  for (int j = 0; j < a.top; ++j) {
-    unsigned long long best = 0;
-    int from = -1;
+  const unsigned long long* src = a.keys + row * total;
+  for (int i = tid; i < total; i += kLpRowThreads) lists[i] = __ldcg(src + i);
+  if (tid < 32) {
+    RowStat r{-INFINITY, 0.f, 0.f};
+    int cnt = 0;
     for (int i = lane; i < a.S; i += 32) {
-      const int h = head[i];
-      const unsigned long long k = h < a.top ? lists[i * a.top + h] : 0ull;
-      if (k > best) { best = k; from = i; }
+      const float4 p = __ldcg(a.part + row * a.S + i);
+      stat_merge(r, RowStat{p.x, p.y, p.z});
+      cnt += __float_as_int(p.w);
     }
-    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
-    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
-    if (from >= 0 && (uint32_t)(best >> 32) == hi && (uint32_t)best == lo) head[from] += 1;
+    r = stat_warp_merge(r);
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
     if (lane == 0) {
-      const bool some = ok && hi != 0u;
-      o.top_ids[row * a.top + j] = some ? (int)~lo : -1;
-      o.top_lp[row * a.top + j] = some ? (logit_of_bits(hi) - r.m) - log_s : ok ? -INFINITY : NAN;
+      const bool ok = stat_valid(r);
+      const float log_s = ok ? logf(r.s) : NAN;
+      const int tok = token_id(a.tokens, row, a.V);
+      const float xt = tok >= 0 ? (float)(static_cast<const T*>(a.logits) + row * a.ld)[tok] : NAN;
+      o.logprob[row] = (xt - r.m) - log_s;
+      o.rank[row] = ok && tok >= 0 ? cnt : -1;
+      o.entropy[row] = ok ? stat_entropy(r) : NAN;
+      max_s = r.m;
+      log_s_s = log_s;
     }
+  }
+  if (a.top == 0) return;
+  __syncthreads();
+  const int d = a.S >= a.top ? 1 : (a.top + a.S - 1) / a.S, r = (a.top + d - 1) / d;
+  for (int i = tid; i < a.S; i += kLpRowThreads) {
+    const unsigned long long h = lists[i * a.top + d - 1];
+    int above = 0;
+    for (int j = 0; j < a.S; ++j) above += lists[j * a.top + d - 1] > h;
+    if (h && above == r - 1) thr_s = h;                // keys are unique: one thread at most
+  }
+  __syncthreads();
+  const unsigned long long thr = thr_s ? thr_s : 1ull; // too few entries: all of them
+  unsigned long long* cand = lists + total;
+  for (int i = tid; i < total; i += kLpRowThreads)
+    if (lists[i] >= thr) cand[atomicAdd(&count_s, 1)] = lists[i];
+  __syncthreads();
+  const int n = count_s;
+  const float M = max_s, log_s = log_s_s;
+  const bool ok = log_s == log_s;
+  for (int i = tid; i < n; i += kLpRowThreads) {
+    const unsigned long long k = cand[i];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += cand[j] > k;
+    if (above < a.top) {
+      o.top_ids[row * a.top + above] = ok ? (int)~(uint32_t)k : -1;
+      o.top_lp[row * a.top + above] = ok ? (logit_of_bits((uint32_t)(k >> 32)) - M) - log_s : NAN;
+    }
+  }
+  for (int i = n + tid; i < a.top; i += kLpRowThreads) {
+    o.top_ids[row * a.top + i] = -1;
+    o.top_lp[row * a.top + i] = ok ? -INFINITY : NAN;
   }
 }
 
@@ -297,7 +350,7 @@ std::vector<torch::Tensor> token_logprobs(torch::Tensor logits, torch::Tensor to
   const int64_t worst = V + vec - 1;                    // a row may start inside a 16-byte piece
   const int64_t small = (int64_t)kLpThreads * 4 * vec;
   const int64_t s4 = (worst + small - 1) / small;
-  const bool u4 = B * s4 <= 2 * 148 && s4 * (8 * top + 4) <= 48 * 1024;
+  const bool u4 = B * s4 <= 2 * 148 && s4 * top * 16 <= 40 * 1024;
   const int64_t per = u4 ? small : 2 * small;
   LpArgs a{};
   a.logits = logits.data_ptr();
@@ -319,7 +372,9 @@ std::vector<torch::Tensor> token_logprobs(torch::Tensor logits, torch::Tensor to
     if (u4) launch_slices<float, 4>(a, (int)B, stream);
     else launch_slices<float, 8>(a, (int)B, stream);
   }
-  const size_t smem = top ? (size_t)a.S * top * 8 + (size_t)a.S * 4 : 0;
+  const size_t smem = (size_t)a.S * top * 16;           // at most 129 slices of 32 keys, twice
+  B200_REQUIRE_CUDA(cudaFuncSetAttribute(bf ? logprob_rows_kernel<__nv_bfloat16> : logprob_rows_kernel<float>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024));
   if (bf) launch_pdl(logprob_rows_kernel<__nv_bfloat16>, dim3((unsigned)B), dim3(kLpRowThreads), smem, stream, a, o);
   else launch_pdl(logprob_rows_kernel<float>, dim3((unsigned)B), dim3(kLpRowThreads), smem, stream, a, o);
   return res;

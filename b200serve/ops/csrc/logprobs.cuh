@@ -26,6 +26,13 @@ __device__ __forceinline__ int token_id(const TokenIds& t, long long row, int V)
   return id >= 0 && id < V ? (int)id : -1;
 }
 
+// 2^x, off by at most 2^-22 of its value
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct RowStat {
   float m, s, t;
 };

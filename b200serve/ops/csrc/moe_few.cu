@@ -41,6 +41,7 @@ constexpr int kMfKb = 4;                         // 64-element blocks per stage
 constexpr int kMfStage = 16 * kMfKb * 128;       // 16 rows: 8 KB
 constexpr int kMfUnits = 16;                     // units announced ahead of the consumers
 constexpr int kMfRed = 2;                        // buffers of partial sums
+constexpr int kMfRouterThreads = 256;
 
 static __device__ int g_mf_err;                  // first error code of the bounded waits, one word per device
 
@@ -61,9 +62,9 @@ struct MfArgs {
 
 // ---------------------------------------------------------------- router logits
 template <int TT>
-__global__ void __launch_bounds__(128) moe_router_kernel(const __nv_bfloat16* __restrict__ router, const MfArgs a,
+__global__ void __launch_bounds__(kMfRouterThreads) moe_router_kernel(const __nv_bfloat16* __restrict__ router, const MfArgs a,
                                                          float* __restrict__ logits, int* __restrict__ counters) {
-  __shared__ float red[4][TT];
+  __shared__ float red[kMfRouterThreads / 32][TT];
   const int e = blockIdx.x, tid = threadIdx.x;
   const __nv_bfloat16* w = router + (size_t)e * a.H;
   bf16x8 first{};                                // a weight: does not depend on the previous kernel
@@ -74,17 +75,20 @@ __global__ void __launch_bounds__(128) moe_router_kernel(const __nv_bfloat16* __
   float acc[TT];
 #pragma unroll
   for (int t = 0; t < TT; ++t) acc[t] = 0.f;
-  for (int i = tid * 8; i < a.H; i += 128 * 8) {
+  for (int i = tid * 8; i < a.H; i += kMfRouterThreads * 8) {
+    const bf16x8 wv = i == tid * 8 ? first : *reinterpret_cast<const bf16x8*>(w + i);
+    bf16x8 xv[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t)                 // rows past T repeat the last one: loads without branches
+      xv[t] = *reinterpret_cast<const bf16x8*>(a.x + min(t, a.T - 1) * a.ldx + i);
     float wf[8];
-    unpack8(i == tid * 8 ? first : *reinterpret_cast<const bf16x8*>(w + i), wf);
+    unpack8(wv, wf);
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      if (t < a.T) {
-        float xf[8];
-        unpack8(*reinterpret_cast<const bf16x8*>(a.x + t * a.ldx + i), xf);
+      float xf[8];
+      unpack8(xv[t], xf);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[t] = fmaf(wf[j], xf[j], acc[t]);
-      }
+      for (int j = 0; j < 8; ++j) acc[t] = fmaf(wf[j], xf[j], acc[t]);
     }
   }
 #pragma unroll
@@ -93,7 +97,12 @@ __global__ void __launch_bounds__(128) moe_router_kernel(const __nv_bfloat16* __
     if ((tid & 31) == 0) red[tid >> 5][t] = s;
   }
   __syncthreads();
-  if (tid < a.T) logits[(size_t)tid * a.E + e] = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+  if (tid < a.T) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMfRouterThreads / 32; ++i) s += red[i][tid];
+    logits[(size_t)tid * a.E + e] = s;
+  }
 }
 
 // ---------------------------------------------------------------- experts
@@ -126,58 +135,63 @@ struct MfShared {
   uint64_t rfull[kMfRed], rempty[kMfRed];
   int unit[kMfUnits];
   int abort_flag;
-  int n_active;
+  int warp_slots[8], warp_pairs[8];              // active experts and pairs among each 32 local experts
   float pair_w[kMfMaxT * kMfMaxK];               // routing weight of an (expert, token) pair
   unsigned char pair_t[kMfMaxT * kMfMaxK];       // its token
   int slot_off[kMfMaxE];                         // first pair of an active expert
   unsigned short slot_e[kMfMaxE], slot_mask[kMfMaxE];   // its local id, its tokens
   unsigned int mask[kMfMaxE];                    // tokens of every local expert
-  float sel_w[kMfMaxT][kMfMaxK];
-  short sel_e[kMfMaxT][kMfMaxK];
 };
 
-// One warp: the k most likely experts of token t and their weights.
-__device__ void route_token(const MfArgs& a, MfShared& sh, int t, int lane) {
+// One warp: the k most likely experts of token t; those on this rank get their bit in sh.mask and their
+// weight in wtab[expert]. EPL: experts per lane.
+template <int EPL>
+__device__ __forceinline__ void route_token(const MfArgs& a, MfShared& sh, float* wtab, int t, int lane) {
   const float* row = a.logits + (size_t)t * a.E;
-  float v[kMfMaxE / 32];
-  uint32_t key[kMfMaxE / 32];                    // order-preserving bits, 0 = absent or taken
+  float p[EPL];
+  uint32_t key[EPL];                             // order-preserving bits, 0 = absent or taken
   float mx = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kMfMaxE / 32; ++i) {
+  for (int i = 0; i < EPL; ++i) {
     const int e = lane + 32 * i;
-    v[i] = e < a.E ? __ldcg(row + e) : -INFINITY;
-    mx = fmaxf(mx, v[i]);
-    const uint32_t u = __float_as_uint(v[i] + 0.f);
+    p[i] = e < a.E ? __ldcg(row + e) : -INFINITY;
+    mx = fmaxf(mx, p[i]);
+    const uint32_t u = __float_as_uint(p[i] + 0.f);
     key[i] = e < a.E ? u ^ ((uint32_t)((int)u >> 31) | 0x80000000u) : 0u;
   }
   mx = warp_max(mx);
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kMfMaxE / 32; ++i) sum += lane + 32 * i < a.E ? __expf(v[i] - mx) : 0.f;
-  sum = warp_sum(sum);
-  float picked = 0.f;
+  for (int i = 0; i < EPL; ++i) {
+    p[i] = lane + 32 * i < a.E ? __expf(p[i] - mx) : 0.f;
+    sum += p[i];
+  }
+  unsigned taken = 0;                            // bit i: this lane's expert i is chosen
   for (int j = 0; j < a.k; ++j) {
-    uint32_t best = 0;
+    uint32_t best = key[0];
     int at = 0;
 #pragma unroll
-    for (int i = 0; i < kMfMaxE / 32; ++i)
+    for (int i = 1; i < EPL; ++i)
       if (key[i] > best) { best = key[i]; at = i; }
     const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-    const int e = (int)__reduce_min_sync(0xffffffffu, best == top ? (unsigned)(lane + 32 * at) : 0xffffffffu);
-    float p = 0.f;
+    const unsigned e = __reduce_min_sync(0xffffffffu, best == top ? (unsigned)(lane + 32 * at) : 0xffffffffu);
 #pragma unroll
-    for (int i = 0; i < kMfMaxE / 32; ++i)
-      if (lane + 32 * i == e) { key[i] = 0u; p = __expf(v[i] - mx); }
-    p = __shfl_sync(0xffffffffu, p, e & 31);
-    picked += p;
-    if (lane == 0) { sh.sel_e[t][j] = (short)e; sh.sel_w[t][j] = p; }
+    for (int i = 0; i < EPL; ++i)
+      if ((unsigned)(lane + 32 * i) == e) { key[i] = 0u; taken |= 1u << i; }
   }
-  const float scale = 1.f / (a.renorm ? picked : sum);
-  __syncwarp();
-  if (lane < a.k) {
-    sh.sel_w[t][lane] *= scale;
-    const int e = sh.sel_e[t][lane] - a.first;
-    if (e >= 0 && e < a.local) atomicOr(&sh.mask[e], 1u << t);
+  if (a.renorm) {
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) sum += taken >> i & 1u ? p[i] : 0.f;
+  }
+  const float scale = 1.f / warp_sum(sum);
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const int e = lane + 32 * i - a.first;
+    if ((taken >> i & 1u) && e >= 0 && e < a.local) {
+      wtab[t * a.local + e] = p[i] * scale;
+      atomicOr(&sh.mask[e], 1u << t);
+    }
   }
 }
 
@@ -208,46 +222,43 @@ __global__ void __launch_bounds__(kMfThreads, 1)
   __syncthreads();
   pdl_wait();
 
-  // ---- routing, the same in every CTA
-  for (int t = warp; t < a.T; t += kMfWarps + 1) route_token(a, sh, t, lane);
-  __syncthreads();
-  if (warp == 0) {
-    int n = 0, pairs = 0;
-    for (int e0 = 0; e0 < a.local; e0 += 32) {
-      const unsigned m = e0 + lane < a.local ? sh.mask[e0 + lane] : 0u;
-      const unsigned some = __ballot_sync(0xffffffffu, m != 0u);
-      int c = __popc(m);
-      int run = c;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int p = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += p;
-      }
-      if (m) {
-        const int s = n + __popc(some & ((1u << lane) - 1u));
-        sh.slot_e[s] = (unsigned short)(e0 + lane);
-        sh.slot_mask[s] = (unsigned short)m;
-        sh.slot_off[s] = pairs + run - c;
-      }
-      n += __popc(some);
-      pairs += __shfl_sync(0xffffffffu, run, 31);
-    }
-    if (lane == 0) sh.n_active = n;
+  // ---- routing, the same in every CTA (the weights of the pairs pass through the partial sums' memory)
+  float* wtab = red;
+  for (int t = warp; t < a.T; t += kMfWarps + 1) {
+    if (a.E <= 32) route_token<1>(a, sh, wtab, t, lane);
+    else if (a.E <= 128) route_token<4>(a, sh, wtab, t, lane);
+    else route_token<8>(a, sh, wtab, t, lane);
   }
   __syncthreads();
-  const int n_active = sh.n_active;
-  // the pairs of every active expert
-  for (int i = tid; i < n_active * a.T; i += kMfThreads) {
-    const int s = i / a.T, t = i % a.T;
-    const unsigned m = sh.slot_mask[s];
-    if (m >> t & 1u) {
-      const int e = sh.slot_e[s] + a.first;
-      float w = 0.f;
-      for (int j = 0; j < a.k; ++j)
-        if (sh.sel_e[t][j] == e) w = sh.sel_w[t][j];
-      const int p = sh.slot_off[s] + __popc(m & ((1u << t) - 1u));
-      sh.pair_w[p] = w;
-      sh.pair_t[p] = (unsigned char)t;
+  // active experts in the order of their id, and their pairs in the order of the tokens
+  const unsigned my_mask = tid < a.local ? sh.mask[tid] : 0u;
+  const unsigned some = __ballot_sync(0xffffffffu, my_mask != 0u);
+  const int mine_n = __popc(my_mask);
+  int run = mine_n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += v;
+  }
+  if (warp < 8 && lane == 31) { sh.warp_slots[warp] = __popc(some); sh.warp_pairs[warp] = run; }
+  __syncthreads();
+  int n_active = 0, slot = 0, off = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (i == warp) { slot = n_active; }
+    if (i < warp) off += sh.warp_pairs[i];
+    n_active += sh.warp_slots[i];
+  }
+  if (my_mask) {
+    slot += __popc(some & ((1u << lane) - 1u));
+    off += run - mine_n;
+    sh.slot_e[slot] = (unsigned short)tid;
+    sh.slot_mask[slot] = (unsigned short)my_mask;
+    sh.slot_off[slot] = off;
+    for (unsigned m = my_mask; m; m &= m - 1u, ++off) {
+      const int t = __ffs(m) - 1;
+      sh.pair_w[off] = wtab[t * a.local + tid];
+      sh.pair_t[off] = (unsigned char)t;
     }
   }
   __syncthreads();
@@ -261,36 +272,48 @@ __global__ void __launch_bounds__(kMfThreads, 1)
     if (lane == 0) {
       // ---------------- producer ----------------
       const uint64_t pol = tc::policy_evict_first();
-      long long st = 0;
+      int slot = 0;
+      uint32_t par = 1;
+      bool live = true;
+      // next free stage: waits for it, announces its bytes, returns its memory
+      auto stage = [&](uint64_t*& bar) -> uint8_t* {
+        live = tc::mbar_wait_bounded(&sh.empty[slot], par, abort_flag, err, 22);
+        bar = &sh.full[slot];
+        uint8_t* dst = ring + slot * kMfStage;
+        if (live) tc::mbar_arrive_expect_tx(bar, kMfStage);
+        if (++slot == kMfStages) { slot = 0; par ^= 1u; }
+        return dst;
+      };
       int u = atomicAdd(a.counters, 1);
-      for (int n = 0;; ++n) {
+      for (int n = 0; live; ++n) {
         const int us = n % kMfUnits;
         if (!tc::mbar_wait_bounded(&sh.uempty[us], ((n / kMfUnits) & 1) ^ 1, abort_flag, err, 21)) break;
         sh.unit[us] = u < total ? u : -1;
         tc::mbar_arrive(&sh.ufull[us]);
         if (u >= total) break;
         const int next = atomicAdd(a.counters, 1);         // needed only at the next unit
-        const int stages = u < n_up ? up_stages : n_active * dn_stages;
-        bool live = true;
-        for (int s = 0; s < stages; ++s, ++st) {
-          const int slot = (int)(st % kMfStages);
-          live = tc::mbar_wait_bounded(&sh.empty[slot], (uint32_t)((st / kMfStages) & 1) ^ 1u, abort_flag, err, 22);
-          if (!live) break;
-          uint8_t* dst = ring + slot * kMfStage;
-          tc::mbar_arrive_expect_tx(&sh.full[slot], kMfStage);
-          if (u < n_up) {
-            // a tile of the gate/up weight: 64 gate rows, then the 64 up rows of the same columns
-            const int cb = u % col_blocks, e = sh.slot_e[u / col_blocks];
-            const int tile = e * (a.I / 64) + cb / 8, r = (cb % 8) * 8;
-            tma_load_4d(dst, &tm_gu, &sh.full[slot], 0, r, s * kMfKb, tile, pol);
-            tma_load_4d(dst + kMfStage / 2, &tm_gu, &sh.full[slot], 0, 64 + r, s * kMfKb, tile, pol);
-          } else {
-            const int hb = u - n_up, e = sh.slot_e[s / dn_stages];
-            tma_load_4d(dst, &tm_dn, &sh.full[slot], 0, (hb % 8) * 16, (s % dn_stages) * kMfKb,
-                        e * a.h_tiles + hb / 8, pol);
+        uint64_t* bar;
+        if (u < n_up) {
+          // a tile of the gate/up weight: 64 gate rows, then the 64 up rows of the same columns
+          const int sl = u / col_blocks, cb = u - sl * col_blocks;
+          const int tile = sh.slot_e[sl] * (a.I / 64) + cb / 8, r = (cb % 8) * 8;
+          for (int kb = 0; kb < a.h_kb && live; kb += kMfKb) {
+            uint8_t* dst = stage(bar);
+            if (!live) break;
+            tma_load_4d(dst, &tm_gu, bar, 0, r, kb, tile, pol);
+            tma_load_4d(dst + kMfStage / 2, &tm_gu, bar, 0, 64 + r, kb, tile, pol);
+          }
+        } else {
+          const int hb = u - n_up, r = (hb % 8) * 16;
+          for (int sl = 0; sl < n_active && live; ++sl) {
+            const int tile = sh.slot_e[sl] * a.h_tiles + hb / 8;
+            for (int kb = 0; kb < a.i_kb && live; kb += kMfKb) {
+              uint8_t* dst = stage(bar);
+              if (!live) break;
+              tma_load_4d(dst, &tm_dn, bar, 0, r, kb, tile, pol);
+            }
           }
         }
-        if (!live) break;
         u = next;
       }
     }
@@ -299,7 +322,9 @@ __global__ void __launch_bounds__(kMfThreads, 1)
     // ---------------- consumers ----------------
     const int g = lane >> 2, t4 = lane & 3;
     const size_t act_rows = (size_t)a.T * a.k;
-    long long st0 = 0;
+    int w0 = 0;                                            // the warp that takes the unit's first stage
+    int slot = warp;                                       // this warp's stages use slots warp, warp + 8, ...
+    uint32_t par = 0;
     bool ready = false;
     for (int n = 0;; ++n) {
       const int us = n % kMfUnits;
@@ -347,13 +372,10 @@ __global__ void __launch_bounds__(kMfThreads, 1)
         }
       }
       bool live = true;
-      int s = (int)((warp - st0 % kMfWarps + kMfWarps) % kMfWarps);
+      int s = (warp - w0) & (kMfWarps - 1);
+      int sl = up ? 0 : s / dn_stages, ks = up ? s : s - sl * dn_stages;
       for (; s < stages; s += kMfWarps) {
-        const long long st = st0 + s;
-        const int slot = (int)(st % kMfStages);
         const uint8_t* w = ring + slot * kMfStage;
-        const uint32_t par = (uint32_t)((st / kMfStages) & 1);
-        const int ks = up ? s : s % dn_stages;
         const int kend = up ? a.H : a.I;
         const uint4 zero = make_uint4(0, 0, 0, 0);
         if (up) {
@@ -376,7 +398,6 @@ __global__ void __launch_bounds__(kMfThreads, 1)
             for (int q = 0; q < NG; ++q) mma_piece(acc[q], lo, hi, b[q][i]);
           }
         } else {
-          const int sl = s / dn_stages;
           const unsigned m = sh.slot_mask[sl];
           const __nv_bfloat16* arow[NG];
 #pragma unroll
@@ -419,6 +440,11 @@ __global__ void __launch_bounds__(kMfThreads, 1)
         }
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&sh.empty[slot]);
+        slot += kMfWarps;
+        if (slot >= kMfStages) { slot = warp; par ^= 1u; }
+        ks += kMfWarps;
+        if (!up)
+          while (ks >= dn_stages) { ks -= dn_stages; ++sl; }
       }
       if (!live) break;
 
@@ -440,10 +466,10 @@ __global__ void __launch_bounds__(kMfThreads, 1)
       if (warp == n % kMfWarps) {
         if (!tc::mbar_wait_bounded(&sh.rfull[rb], rpar, abort_flag, err, 27)) break;
         const float* part = red + rb * kMfWarps * NG * 128;
-        const int w0 = (int)(st0 % kMfWarps), nw = min(stages, kMfWarps);
+        const int nw = min(stages, kMfWarps);
         auto total_of = [&](int idx) {                     // partial sums in stage order
           float v = 0.f;
-          for (int i = 0; i < nw; ++i) v += part[((w0 + i) % kMfWarps) * NG * 128 + idx];
+          for (int i = 0; i < nw; ++i) v += part[((w0 + i) & (kMfWarps - 1)) * NG * 128 + idx];
           return v;
         };
         if (up) {
@@ -472,7 +498,7 @@ __global__ void __launch_bounds__(kMfThreads, 1)
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&sh.rempty[rb]);
       }
-      st0 += stages;
+      w0 = (w0 + stages) & (kMfWarps - 1);
     }
   }
   __syncthreads();
@@ -550,7 +576,7 @@ void moe_layer(torch::Tensor x, torch::Tensor router, torch::Tensor gate_up, int
   const CUtensorMap td = tma_bf16(down.data_ptr(), 4, dn_dims, dn_str, dn_box);
   auto stream = at::cuda::getCurrentCUDAStream();
   const __nv_bfloat16* rp = reinterpret_cast<const __nv_bfloat16*>(router.data_ptr());
-  const dim3 rg((unsigned)E), rb(128);
+  const dim3 rg((unsigned)E), rb(kMfRouterThreads);
   if (T <= 1) launch_pdl(moe_router_kernel<1>, rg, rb, 0, stream, rp, a, logits, a.counters);
   else if (T <= 4) launch_pdl(moe_router_kernel<4>, rg, rb, 0, stream, rp, a, logits, a.counters);
   else if (T <= 8) launch_pdl(moe_router_kernel<8>, rg, rb, 0, stream, rp, a, logits, a.counters);
