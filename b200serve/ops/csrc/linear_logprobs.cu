@@ -180,14 +180,14 @@ __global__ void __launch_bounds__(kLlThreads, 1)
     const float L2E = 1.4426950408889634f;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
       const LlUnit x = ll_unit(a, u);
       const int row = x.m0 + quad * 32 + lane;
       const int cols = min(x.n - half * kLlCols, kLlCols); // <= 0: this half of a narrow tile has none
       float v[kLlCols];
       bool live = true;
       for (int k0 = 0; k0 < a.kb_total; k0 += kLlPart) {
-        live = tc::mbar_wait_bounded(&tfull[acc], acc_phase, abort_flag, err, 14);
+        live = __all_sync(0xffffffffu, tc::mbar_wait_bounded(&tfull[acc], acc_phase, abort_flag, err, 14));
         if (!live) break;
         tc::tc_fence_after();
         const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * kLlBN + half * kLlCols;

@@ -5,19 +5,23 @@
 // With so few rows the layer is the read of the chosen experts' weights, 6 H I bytes each, and
 // what costs besides is every wait between dependent steps. So:
 //   * moe_router: one CTA per expert row of R computes its logit for every token.
-//   * moe_few: one CTA per SM. Every CTA repeats the tiny routing step for itself, then takes units
-//     of work from one counter: first all gate/up units (8 inner columns of one expert: 8
-//     gate and 8 up rows), then all down units (16 output rows over every chosen expert). Its
-//     producer thread runs up to 24 stages (192 KB) ahead with TMA, across units and from the
-//     gate/up part into the down part, so the memory pipe does not drain where the
-//     down products wait for the activations. Units are handed out in order and a gate/up unit
-//     waits for nothing but memory, so the down units' wait ends however few CTAs run at a time.
+//   * moe_few: two CTAs of eight warps per SM. Every CTA repeats the tiny routing step for itself,
+//     then takes units of work from one counter: first all gate/up units (8 inner columns of one
+//     expert: 8 gate and 8 up rows), then all down units (16 output rows over every chosen
+//     expert). The warps share a unit's sum over k, 128 elements (a chunk, 4 KB of weights) at a
+//     time, and keep the weights of their next chunks on the way with cp.async, across units and from
+//     the gate/up part into the down part, so the memory pipe does not drain while the down
+//     products wait for the activations. Units are handed out in order and a gate/up unit waits for
+//     nothing but memory, so the down units' wait ends however few CTAs run at a time.
 //
-// Products: mma.sync m16n8k16 with the weight rows as M and the tokens as N (8 per group). The
-// tensor pipe is a few percent busy; tcgen05 tiles of 128 weight rows would only coarsen the units
-// that balance the SMs. Lane (g, t) of a fragment takes 16 bytes of row g at element 16 t + 8 h
-// of a 64-element block: the sum over k may run in any order as long as weights and activations
-// agree on it, and with the TMA's 128-byte swizzle these reads have no bank conflicts.
+// Products: mma.sync m16n8k16 with the weight rows as M and the tokens as N (8 per group). A lane copies
+// into shared memory just the bytes that it reads back itself, so a ring of chunks takes neither
+// barriers nor registers: lane (g, t) takes 16 bytes of rows g and g + 8 at element
+// 32 h + 8 t of a 64-element block (the sum over k may run in any order that weights and activations
+// agree on), so a warp's load covers eight whole 64-byte pieces. The tensor pipe is a few percent
+// busy; tcgen05 tiles of 128 weight rows would only coarsen the units that balance the SMs. TMA
+// into shared memory was slower here: boxes of 8 rows and the waits on 24 stages took 0.25 us per
+// 8 KB and SM, 218 us where this takes 169 (16 rows, 128 experts of 768, top 8, 2048 wide).
 //
 // Numerics: fp32 accumulation; the routing weight is folded into the activation in fp32, and the
 // activation is kept as the sum of two bf16 (high part and remainder, 16 bits of mantissa), so
@@ -28,19 +32,13 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <algorithm>
-#include "tc_primitives.cuh"
 #include "tma_host.h"
 
 namespace b200 {
 
 constexpr int kMfMaxT = 16, kMfMaxK = 16, kMfMaxE = 256;
-constexpr int kMfWarps = 8;                      // consumer warps; warp 8 is the producer
-constexpr int kMfThreads = (kMfWarps + 1) * 32;
-constexpr int kMfStages = 24;                    // a multiple of kMfWarps: a slot is always the same warp's
-constexpr int kMfKb = 4;                         // 64-element blocks per stage
-constexpr int kMfStage = 16 * kMfKb * 128;       // 16 rows: 8 KB
-constexpr int kMfUnits = 16;                     // units announced ahead of the consumers
-constexpr int kMfRed = 2;                        // buffers of partial sums
+constexpr int kMfWarps = 8;
+constexpr int kMfThreads = kMfWarps * 32;
 constexpr int kMfRouterThreads = 256;
 
 static __device__ int g_mf_err;                  // first error code of the bounded waits, one word per device
@@ -106,15 +104,6 @@ __global__ void __launch_bounds__(kMfRouterThreads) moe_router_kernel(const __nv
 }
 
 // ---------------------------------------------------------------- experts
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
-                                            int c3, uint64_t hint) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(tc::smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(hint)
-      : "memory");
-}
-
 __device__ __forceinline__ void mma_16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
   asm volatile(
@@ -129,13 +118,13 @@ __device__ __forceinline__ void mma_piece(float* d, const uint4& lo, const uint4
   mma_16816(d, lo.z, hi.z, lo.w, hi.w, b.z, b.w);
 }
 
+template <int NG>
 struct MfShared {
-  uint64_t full[kMfStages], empty[kMfStages];
-  uint64_t ufull[kMfUnits], uempty[kMfUnits];
-  uint64_t rfull[kMfRed], rempty[kMfRed];
-  int unit[kMfUnits];
-  int abort_flag;
-  int warp_slots[8], warp_pairs[8];              // active experts and pairs among each 32 local experts
+  static constexpr int kDepth = NG == 1 ? 3 : 2;  // chunks on the way per warp; two CTAs share 227 KB
+  uint4 ring[kDepth][8][kMfThreads];             // [chunk][block, half, rows g or g + 8][thread]
+  float red[2][kMfWarps][NG * 128];              // partial sums: two units' worth
+  int unit[4];                                   // the CTA's units, a ring
+  int warp_slots[kMfWarps], warp_pairs[kMfWarps];  // active experts and pairs among each 32 local experts
   float pair_w[kMfMaxT * kMfMaxK];               // routing weight of an (expert, token) pair
   unsigned char pair_t[kMfMaxT * kMfMaxK];       // its token
   int slot_off[kMfMaxE];                         // first pair of an active expert
@@ -143,10 +132,10 @@ struct MfShared {
   unsigned int mask[kMfMaxE];                    // tokens of every local expert
 };
 
-// One warp: the k most likely experts of token t; those on this rank get their bit in sh.mask and their
-// weight in wtab[expert]. EPL: experts per lane.
+// One warp: the k most likely experts of token t; those on this rank get their bit in mask[expert] and their
+// weight in wtab[t][expert]. EPL: experts per lane.
 template <int EPL>
-__device__ __forceinline__ void route_token(const MfArgs& a, MfShared& sh, float* wtab, int t, int lane) {
+__device__ __forceinline__ void route_token(const MfArgs& a, unsigned int* mask, float* wtab, int t, int lane) {
   const float* row = a.logits + (size_t)t * a.E;
   float p[EPL];
   uint32_t key[EPL];                             // order-preserving bits, 0 = absent or taken
@@ -190,44 +179,35 @@ __device__ __forceinline__ void route_token(const MfArgs& a, MfShared& sh, float
     const int e = lane + 32 * i - a.first;
     if ((taken >> i & 1u) && e >= 0 && e < a.local) {
       wtab[t * a.local + e] = p[i] * scale;
-      atomicOr(&sh.mask[e], 1u << t);
+      atomicOr(&mask[e], 1u << t);
     }
   }
 }
 
-// NG: groups of 8 tokens
-template <int NG>
-__global__ void __launch_bounds__(kMfThreads, 1)
-    moe_few_kernel(const __grid_constant__ CUtensorMap tm_gu, const __grid_constant__ CUtensorMap tm_dn,
-                   const MfArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* red = reinterpret_cast<float*>(ring + kMfStages * kMfStage);      // [kMfRed][warps][NG * 128]
-  MfShared& sh = *reinterpret_cast<MfShared*>(red + kMfRed * kMfWarps * NG * 128);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  volatile int* abort_flag = &sh.abort_flag;
-  int* err = &g_mf_err;
-
-  if (tid == 0) {
-    for (int s = 0; s < kMfStages; ++s) { tc::mbar_init(&sh.full[s], 1); tc::mbar_init(&sh.empty[s], 1); }
-    for (int s = 0; s < kMfUnits; ++s) { tc::mbar_init(&sh.ufull[s], 1); tc::mbar_init(&sh.uempty[s], kMfWarps); }
-    for (int s = 0; s < kMfRed; ++s) { tc::mbar_init(&sh.rfull[s], kMfWarps); tc::mbar_init(&sh.rempty[s], 1); }
-    sh.abort_flag = 0;
-    tc::fence_barrier_init();
-    tc::fence_proxy_async_smem();
-    tc::prefetch_tmap(&tm_gu);
-    tc::prefetch_tmap(&tm_dn);
-  }
+// NG: groups of 8 tokens. PAIR (at most 4 tokens): the down products take the activations' high parts in
+// columns 0..3 and their remainders in columns 4..7 of the one group.
+template <int NG, bool PAIR>
+__global__ void __launch_bounds__(kMfThreads, 2)
+    moe_few_kernel(const __nv_bfloat16* __restrict__ gate_up, const __nv_bfloat16* __restrict__ down, const MfArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  MfShared<NG>& sh = *reinterpret_cast<MfShared<NG>*>(smem_raw);
+  constexpr int DEPTH = MfShared<NG>::kDepth;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   for (int e = tid; e < a.local; e += kMfThreads) sh.mask[e] = 0u;
   __syncthreads();
   pdl_wait();
+  if (tid == 0) {
+    sh.unit[0] = atomicAdd(a.counters, 1);
+    sh.unit[1] = atomicAdd(a.counters, 1);
+  }
 
   // ---- routing, the same in every CTA (the weights of the pairs pass through the partial sums' memory)
-  float* wtab = red;
-  for (int t = warp; t < a.T; t += kMfWarps + 1) {
-    if (a.E <= 32) route_token<1>(a, sh, wtab, t, lane);
-    else if (a.E <= 128) route_token<4>(a, sh, wtab, t, lane);
-    else route_token<8>(a, sh, wtab, t, lane);
+  static_assert(sizeof(sh.red) >= (NG == 1 ? 8 : 16) * kMfMaxE * 4, "the routing weights must fit");
+  float* wtab = &sh.red[0][0][0];
+  for (int t = warp; t < a.T; t += kMfWarps) {
+    if (a.E <= 32) route_token<1>(a, sh.mask, wtab, t, lane);
+    else if (a.E <= 128) route_token<4>(a, sh.mask, wtab, t, lane);
+    else route_token<8>(a, sh.mask, wtab, t, lane);
   }
   __syncthreads();
   // active experts in the order of their id, and their pairs in the order of the tokens
@@ -240,21 +220,21 @@ __global__ void __launch_bounds__(kMfThreads, 1)
     const int v = __shfl_up_sync(0xffffffffu, run, o);
     if (lane >= o) run += v;
   }
-  if (warp < 8 && lane == 31) { sh.warp_slots[warp] = __popc(some); sh.warp_pairs[warp] = run; }
+  if (lane == 31) { sh.warp_slots[warp] = __popc(some); sh.warp_pairs[warp] = run; }
   __syncthreads();
-  int n_active = 0, slot = 0, off = 0;
+  int n_active = 0, first_slot = 0, off = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (i == warp) { slot = n_active; }
+  for (int i = 0; i < kMfWarps; ++i) {
+    if (i == warp) first_slot = n_active;
     if (i < warp) off += sh.warp_pairs[i];
     n_active += sh.warp_slots[i];
   }
   if (my_mask) {
-    slot += __popc(some & ((1u << lane) - 1u));
+    const int sl = first_slot + __popc(some & ((1u << lane) - 1u));
     off += run - mine_n;
-    sh.slot_e[slot] = (unsigned short)tid;
-    sh.slot_mask[slot] = (unsigned short)my_mask;
-    sh.slot_off[slot] = off;
+    sh.slot_e[sl] = (unsigned short)tid;
+    sh.slot_mask[sl] = (unsigned short)my_mask;
+    sh.slot_off[sl] = off;
     for (unsigned m = my_mask; m; m &= m - 1u, ++off) {
       const int t = __ffs(m) - 1;
       sh.pair_w[off] = wtab[t * a.local + tid];
@@ -266,246 +246,216 @@ __global__ void __launch_bounds__(kMfThreads, 1)
   const int col_blocks = a.I / 8;                          // gate/up units per expert
   const int n_up = n_active * col_blocks;
   const int total = n_up + (a.H + 15) / 16;
-  const int up_stages = (a.h_kb + kMfKb - 1) / kMfKb, dn_stages = (a.i_kb + kMfKb - 1) / kMfKb;
+  const int up_chunks = (a.h_kb + 1) / 2, dn_chunks = (a.i_kb + 1) / 2;   // per unit; per unit and expert
+  const size_t act_rows = (size_t)a.T * a.k;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  // Offsets in 16-byte words: a 64-element row of a weight tile has 8, a tile 1024.
+  const int lane_off = g * 8 + t4;
 
-  if (warp == kMfWarps) {
-    if (lane == 0) {
-      // ---------------- producer ----------------
-      const uint64_t pol = tc::policy_evict_first();
-      int slot = 0;
-      uint32_t par = 1;
-      bool live = true;
-      // next free stage: waits for it, announces its bytes, returns its memory
-      auto stage = [&](uint64_t*& bar) -> uint8_t* {
-        live = tc::mbar_wait_bounded(&sh.empty[slot], par, abort_flag, err, 22);
-        bar = &sh.full[slot];
-        uint8_t* dst = ring + slot * kMfStage;
-        if (live) tc::mbar_arrive_expect_tx(bar, kMfStage);
-        if (++slot == kMfStages) { slot = 0; par ^= 1u; }
-        return dst;
-      };
-      int u = atomicAdd(a.counters, 1);
-      for (int n = 0; live; ++n) {
-        const int us = n % kMfUnits;
-        if (!tc::mbar_wait_bounded(&sh.uempty[us], ((n / kMfUnits) & 1) ^ 1, abort_flag, err, 21)) break;
-        sh.unit[us] = u < total ? u : -1;
-        tc::mbar_arrive(&sh.ufull[us]);
-        if (u >= total) break;
-        const int next = atomicAdd(a.counters, 1);         // needed only at the next unit
-        uint64_t* bar;
-        if (u < n_up) {
-          // a tile of the gate/up weight: 64 gate rows, then the 64 up rows of the same columns
-          const int sl = u / col_blocks, cb = u - sl * col_blocks;
-          const int tile = sh.slot_e[sl] * (a.I / 64) + cb / 8, r = (cb % 8) * 8;
-          for (int kb = 0; kb < a.h_kb && live; kb += kMfKb) {
-            uint8_t* dst = stage(bar);
-            if (!live) break;
-            tma_load_4d(dst, &tm_gu, bar, 0, r, kb, tile, pol);
-            tma_load_4d(dst + kMfStage / 2, &tm_gu, bar, 0, 64 + r, kb, tile, pol);
-          }
-        } else {
-          const int hb = u - n_up, r = (hb % 8) * 16;
-          for (int sl = 0; sl < n_active && live; ++sl) {
-            const int tile = sh.slot_e[sl] * a.h_tiles + hb / 8;
-            for (int kb = 0; kb < a.i_kb && live; kb += kMfKb) {
-              uint8_t* dst = stage(bar);
-              if (!live) break;
-              tma_load_4d(dst, &tm_dn, bar, 0, r, kb, tile, pol);
-            }
-          }
-        }
-        u = next;
-      }
+  // ---- the next chunk that this warp copies: chunk `nc` of unit `nu`, which is the CTA's `nn`-th; `ahead` chunks
+  // are copied and not consumed
+  int nn = 0, nu = sh.unit[0], nc = warp, nsl = 0, nks = 0, n_chunks = 0, in_slot = 0, out_slot = 0, ahead = 0;
+  const uint4* n_base = nullptr;                           // tile of the unit (down: of expert 0, row block included)
+  int n_hi = 0, n_kb = 0;
+  auto enter = [&]() {                                     // sets up unit nu
+    nc = warp;
+    if (nu < n_up) {
+      const int sl = nu / col_blocks, cb = nu - sl * col_blocks;
+      n_base = reinterpret_cast<const uint4*>(gate_up) +
+               ((size_t)(sh.slot_e[sl] * (a.I / 64) + cb / 8) * a.h_kb * 128 + (cb % 8) * 8) * 8 + lane_off;
+      n_hi = 64 * 8;                                       // a tile: 64 gate rows, then the 64 up rows of the same columns
+      n_kb = a.h_kb;
+      n_chunks = up_chunks;
+      nsl = 0;
+      nks = warp;
+    } else if (nu < total) {
+      const int hb = nu - n_up;
+      n_base = reinterpret_cast<const uint4*>(down) + ((size_t)(hb / 8) * a.i_kb * 128 + (hb % 8) * 16) * 8 + lane_off;
+      n_hi = 8 * 8;
+      n_kb = a.i_kb;
+      n_chunks = n_active * dn_chunks;
+      nsl = warp / dn_chunks;
+      nks = warp - nsl * dn_chunks;
+    } else {
+      n_chunks = 0;
     }
-    __syncwarp();
-  } else {
-    // ---------------- consumers ----------------
-    const int g = lane >> 2, t4 = lane & 3;
-    const size_t act_rows = (size_t)a.T * a.k;
-    int w0 = 0;                                            // the warp that takes the unit's first stage
-    int slot = warp;                                       // this warp's stages use slots warp, warp + 8, ...
-    uint32_t par = 0;
-    bool ready = false;
-    for (int n = 0;; ++n) {
-      const int us = n % kMfUnits;
-      if (!tc::mbar_wait_bounded(&sh.ufull[us], (n / kMfUnits) & 1, abort_flag, err, 23)) break;
-      const int u = *(volatile int*)&sh.unit[us];
-      if (u < 0) break;
-      const bool up = u < n_up;
-      const int stages = up ? up_stages : n_active * dn_stages;
-      const int us_slot = up ? u / col_blocks : 0;
-      const int ntok = up ? __popc(sh.slot_mask[us_slot]) : a.T;
-      float acc[NG][4];
+  };
+  // copies until DEPTH chunks are ahead or the units known (up to the CTA's `known`-th) hold no more
+  auto fill = [&](int known) {
+    while (ahead < DEPTH) {
+      if (nc >= n_chunks) {
+        if (nn == known) return;
+        ++nn;
+        nu = sh.unit[nn & 3];
+        enter();
+        continue;
+      }
+      const uint4* base = n_base;
+      if (nu >= n_up) base += (size_t)sh.slot_e[nsl] * a.h_tiles * a.i_kb * 1024;
 #pragma unroll
-      for (int q = 0; q < NG; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[q][i] = 0.f;
+      for (int i = 0; i < 8; ++i) {
+        const int kb = nks * 2 + (i >> 2);
+        const uint4* src = base + (size_t)min(kb, n_kb - 1) * 1024 + (i >> 1 & 1) * 4 + ((i & 1) ? n_hi : 0);
+        const int bytes = kb < n_kb ? 16 : 0;              // past the last block: zeros
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                         (uint32_t)__cvta_generic_to_shared(&sh.ring[in_slot][i][tid])), "l"(src), "r"(bytes)
+                     : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      in_slot = in_slot + 1 == DEPTH ? 0 : in_slot + 1;
+      ++ahead;
+      nc += kMfWarps;
+      nks += kMfWarps;
+      if (nu >= n_up)
+        while (nks >= dn_chunks) { nks -= dn_chunks; ++nsl; }
+    }
+  };
+  enter();
+  fill(1);
 
-      if (!up && !ready && stages > 0) {
-        // the activations of every gate/up unit (one counter: by the time a down unit comes up the
-        // gate/up units are done or in flight)
-        if (lane == 0) {
+  bool ready = false;
+  int done_units = 0;                                      // gate/up units of this CTA
+  for (int n = 0;; ++n) {
+    const int u = sh.unit[n & 3];
+    const bool up = u < n_up;
+    if (!up && !ready) {
+      // every warp's activations are written: publish the CTA's units, then wait for everybody's
+      __syncthreads();
+      if (tid == 0) {
+        __threadfence();
+        if (done_units) atomicAdd(a.counters + 1, done_units);
+        if (u < total && n_active > 0) {
           const uint64_t deadline = globaltimer_ns() + 2000000000ull;
           for (uint32_t it = 1;; ++it) {
             int done;
             asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(done) : "l"(a.counters + 1) : "memory");
-            if (done >= n_up || *abort_flag) break;
+            if (done >= n_up) break;
             if ((it & 63u) == 0 && globaltimer_ns() > deadline) {
-              atomicExch(err, 24);
-              *abort_flag = 1;
+              atomicExch(&g_mf_err, 24);                   // reported by moe_layer_error(); the results are void
               break;
             }
           }
         }
-        __syncwarp();
-        if (*abort_flag) break;
-        ready = true;
       }
+      __syncthreads();
+      ready = true;
+    }
+    if (u >= total) break;
+    // the unit after next: asked for now, needed at the end of this one
+    int ticket = 0;
+    if (tid == 0) ticket = atomicAdd(a.counters, 1);
 
-      // the token of this lane's column in the gate/up part: the g-th of the expert's tokens
-      const __nv_bfloat16* xrow[NG];
+    const int us = up ? u / col_blocks : 0;
+    const int ntok = up ? __popc(sh.slot_mask[us]) : a.T;
+    const int chunks = up ? up_chunks : n_active * dn_chunks;
+    const __nv_bfloat16* xrow[NG];                         // the token of this lane's column: the g-th of the expert's
+    if (up) {
+#pragma unroll
+      for (int q = 0; q < NG; ++q) {
+        const int c = q * 8 + g;
+        xrow[q] = c < ntok ? a.x + sh.pair_t[sh.slot_off[us] + c] * a.ldx : nullptr;
+      }
+    }
+    // two accumulators per group keep the chain of dependent MMAs short
+    float acc[NG][2][4];
+#pragma unroll
+    for (int q = 0; q < NG; ++q)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[q][i >> 2][i & 3] = 0.f;
+
+    int sl = up ? 0 : warp / dn_chunks, ks = warp - sl * dn_chunks;
+    for (int c = warp; c < chunks; c += kMfWarps) {
+      fill(n + 1);
+      // the oldest chunk has landed once at most ahead - 1 groups are on the way
+      if (ahead >= 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else if (ahead == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else asm volatile("cp.async.wait_group 0;" ::: "memory");
+      uint4 w[2][2][2];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i >> 2][i >> 1 & 1][i & 1] = sh.ring[out_slot][i][tid];
+      const int k0 = ks * 128 + 8 * t4;
       if (up) {
 #pragma unroll
         for (int q = 0; q < NG; ++q) {
-          const int c = q * 8 + g;
-          xrow[q] = c < ntok ? a.x + sh.pair_t[sh.slot_off[us_slot] + c] * a.ldx : nullptr;
+          if (q * 8 >= ntok) break;
+          uint4 b[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            b[i] = xrow[q] != nullptr && k0 + 32 * i < a.H ? *reinterpret_cast<const uint4*>(xrow[q] + k0 + 32 * i)
+                                                           : zero;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mma_piece(acc[q][i & 1], w[i >> 1][i & 1][0], w[i >> 1][i & 1][1], b[i]);
+        }
+      } else {
+        const unsigned m = sh.slot_mask[sl];
+#pragma unroll
+        for (int q = 0; q < NG; ++q) {
+          if (!(m >> (8 * q) & 0xffu)) continue;           // none of this group's tokens
+          const int t = PAIR ? g & 3 : q * 8 + g;
+          const __nv_bfloat16* arow = a.act + (size_t)(sh.slot_off[sl] + __popc(m & ((1u << t) - 1u))) * a.I + k0;
+          if (PAIR && g >= 4) arow += act_rows * a.I;
+          const bool in = m >> t & 1u;
+          constexpr int PARTS = PAIR ? 1 : 2;              // high parts, remainders
+          uint4 b[PARTS][4];
+#pragma unroll
+          for (int j = 0; j < PARTS; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              b[j][i] = in && k0 + 32 * i < a.I ? *reinterpret_cast<const uint4*>(arow + j * act_rows * a.I + 32 * i)
+                                                : zero;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < PARTS; ++j)
+              mma_piece(acc[q][PARTS == 1 ? i & 1 : j], w[i >> 1][i & 1][0], w[i >> 1][i & 1][1], b[j][i]);
         }
       }
-      bool live = true;
-      int s = (warp - w0) & (kMfWarps - 1);
-      int sl = up ? 0 : s / dn_stages, ks = up ? s : s - sl * dn_stages;
-      for (; s < stages; s += kMfWarps) {
-        const uint8_t* w = ring + slot * kMfStage;
-        const int kend = up ? a.H : a.I;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        if (up) {
-          uint4 b[NG][2 * kMfKb];                          // activations do not wait for the weights
-#pragma unroll
-          for (int q = 0; q < NG; ++q)
-#pragma unroll
-            for (int i = 0; i < 2 * kMfKb; ++i) {
-              const int k0 = (ks * kMfKb + i / 2) * 64 + 16 * t4 + 8 * (i & 1);
-              b[q][i] = xrow[q] != nullptr && k0 < kend ? *reinterpret_cast<const uint4*>(xrow[q] + k0) : zero;
-            }
-          live = tc::mbar_wait_bounded(&sh.full[slot], par, abort_flag, err, 25);
-          if (!live) break;
-#pragma unroll
-          for (int i = 0; i < 2 * kMfKb; ++i) {
-            const uint8_t* p = w + (i / 2) * 1024 + g * 128 + (((2 * t4 + (i & 1)) ^ g) << 4);
-            const uint4 lo = *reinterpret_cast<const uint4*>(p);
-            const uint4 hi = *reinterpret_cast<const uint4*>(p + kMfStage / 2);
-#pragma unroll
-            for (int q = 0; q < NG; ++q) mma_piece(acc[q], lo, hi, b[q][i]);
-          }
-        } else {
-          const unsigned m = sh.slot_mask[sl];
-          const __nv_bfloat16* arow[NG];
-#pragma unroll
-          for (int q = 0; q < NG; ++q) {
-            const int t = q * 8 + g;
-            arow[q] = m >> t & 1u
-                          ? a.act + (size_t)(sh.slot_off[sl] + __popc(m & ((1u << t) - 1u))) * a.I
-                          : nullptr;
-          }
-          constexpr int HALF = kMfKb / NG;                 // blocks whose activations are loaded at a time
-#pragma unroll
-          for (int part = 0; part < NG; ++part) {
-            uint4 b[NG][2][2 * HALF];
-#pragma unroll
-            for (int q = 0; q < NG; ++q)
-#pragma unroll
-              for (int i = 0; i < 2 * HALF; ++i) {
-                const int k0 = (ks * kMfKb + part * HALF + i / 2) * 64 + 16 * t4 + 8 * (i & 1);
-                const bool in = arow[q] != nullptr && k0 < kend;
-                b[q][0][i] = in ? *reinterpret_cast<const uint4*>(arow[q] + k0) : zero;
-                b[q][1][i] = in ? *reinterpret_cast<const uint4*>(arow[q] + act_rows * a.I + k0) : zero;
-              }
-            if (part == 0) {
-              live = tc::mbar_wait_bounded(&sh.full[slot], par, abort_flag, err, 25);
-              if (!live) break;
-            }
-#pragma unroll
-            for (int i = 0; i < 2 * HALF; ++i) {
-              const uint8_t* p = w + (part * HALF + i / 2) * 2048 + g * 128 + (((2 * t4 + (i & 1)) ^ g) << 4);
-              const uint4 lo = *reinterpret_cast<const uint4*>(p);
-              const uint4 hi = *reinterpret_cast<const uint4*>(p + 1024);
-#pragma unroll
-              for (int q = 0; q < NG; ++q) {
-                mma_piece(acc[q], lo, hi, b[q][0][i]);
-                mma_piece(acc[q], lo, hi, b[q][1][i]);
-              }
-            }
-          }
-          if (!live) break;
-        }
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sh.empty[slot]);
-        slot += kMfWarps;
-        if (slot >= kMfStages) { slot = warp; par ^= 1u; }
-        ks += kMfWarps;
-        if (!up)
-          while (ks >= dn_stages) { ks -= dn_stages; ++sl; }
-      }
-      if (!live) break;
-
-      // ---- join the warps' partial sums; one warp in turn finishes the unit
-      const int rb = n % kMfRed;
-      const uint32_t rpar = (uint32_t)((n / kMfRed) & 1);
-      if (!tc::mbar_wait_bounded(&sh.rempty[rb], rpar ^ 1u, abort_flag, err, 26)) break;
-      float* mine = red + (rb * kMfWarps + warp) * NG * 128;
-#pragma unroll
-      for (int q = 0; q < NG; ++q) {
-        *reinterpret_cast<float2*>(mine + q * 128 + g * 8 + 2 * t4) = make_float2(acc[q][0], acc[q][1]);
-        *reinterpret_cast<float2*>(mine + q * 128 + (g + 8) * 8 + 2 * t4) = make_float2(acc[q][2], acc[q][3]);
-      }
-      __syncwarp();
-      if (lane == 0) {
-        tc::mbar_arrive(&sh.rfull[rb]);
-        tc::mbar_arrive(&sh.uempty[us]);
-      }
-      if (warp == n % kMfWarps) {
-        if (!tc::mbar_wait_bounded(&sh.rfull[rb], rpar, abort_flag, err, 27)) break;
-        const float* part = red + rb * kMfWarps * NG * 128;
-        const int nw = min(stages, kMfWarps);
-        auto total_of = [&](int idx) {                     // partial sums in stage order
-          float v = 0.f;
-          for (int i = 0; i < nw; ++i) v += part[((w0 + i) & (kMfWarps - 1)) * NG * 128 + idx];
-          return v;
-        };
-        if (up) {
-          const int cb = u % col_blocks, off = sh.slot_off[us_slot];
-          for (int i = lane; i < ntok * 8; i += 32) {
-            const int c = i & 7, p = i >> 3;               // inner column, token of the expert
-            const int idx = (p >> 3) * 128 + c * 8 + (p & 7);
-            const float gate = total_of(idx), upv = total_of(idx + 64);
-            const float v = gate / (1.f + __expf(-gate)) * upv * sh.pair_w[off + p];
-            const __nv_bfloat16 h = __float2bfloat16_rn(v);
-            __nv_bfloat16* dst = a.act + (size_t)(off + p) * a.I + cb * 8 + c;
-            dst[0] = h;
-            dst[act_rows * a.I] = __float2bfloat16_rn(v - __bfloat162float(h));
-          }
-          __threadfence();
-          __syncwarp();
-          if (lane == 0) atomicAdd(a.counters + 1, 1);
-        } else {
-          const int h0 = (u - n_up) * 16;
-          for (int i = lane; i < a.T * 16; i += 32) {
-            const int r = i & 15, t = i >> 4;
-            if (h0 + r < a.H)
-              a.out[t * a.ldo + h0 + r] = __float2bfloat16_rn(total_of((t >> 3) * 128 + r * 8 + (t & 7)));
-          }
-        }
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sh.rempty[rb]);
-      }
-      w0 = (w0 + stages) & (kMfWarps - 1);
+      out_slot = out_slot + 1 == DEPTH ? 0 : out_slot + 1;
+      --ahead;
+      ks += kMfWarps;
+      if (!up)
+        while (ks >= dn_chunks) { ks -= dn_chunks; ++sl; }
     }
-  }
-  __syncthreads();
-  if (*abort_flag) {
-    // error path: give TMA copies that may still be landing in shared memory time to finish
-    const uint64_t until = globaltimer_ns() + 100000ull;
-    while (globaltimer_ns() < until) {
+    fill(n + 1);                                           // under the join and the next unit's start
+
+    // ---- join the warps' partial sums, in the order of the warps
+    float(*red)[NG * 128] = sh.red[n & 1];
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      const float* c0 = acc[q][0];
+      const float* c1 = acc[q][1];
+      float* mine = red[warp] + q * 128;
+      *reinterpret_cast<float2*>(mine + g * 8 + 2 * t4) = make_float2(c0[0] + c1[0], c0[1] + c1[1]);
+      *reinterpret_cast<float2*>(mine + (g + 8) * 8 + 2 * t4) = make_float2(c0[2] + c1[2], c0[3] + c1[3]);
+    }
+    if (tid == 0) sh.unit[(n + 2) & 3] = ticket;
+    __syncthreads();
+    auto sum_of = [&](int idx) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < kMfWarps; ++i) v += red[i][idx];
+      return v;
+    };
+    if (up) {
+      ++done_units;
+      const int c = tid & 7, p = tid >> 3;                 // inner column, token of the expert
+      if (p < ntok) {
+        const int idx = (p >> 3) * 128 + c * 8 + (p & 7), pair = sh.slot_off[us] + p;
+        const float gate = sum_of(idx), upv = sum_of(idx + 64);
+        const float v = gate / (1.f + __expf(-gate)) * upv * sh.pair_w[pair];
+        const __nv_bfloat16 h = __float2bfloat16_rn(v);
+        __nv_bfloat16* dst = a.act + (size_t)pair * a.I + (u - us * col_blocks) * 8 + c;
+        dst[0] = h;
+        dst[act_rows * a.I] = __float2bfloat16_rn(v - __bfloat162float(h));
+      }
+    } else {
+      const int r = tid & 15, t = tid >> 4, h = (u - n_up) * 16 + r;   // output row, token
+      if (t < a.T && h < a.H) {
+        const int idx = (t >> 3) * 128 + r * 8 + (t & 7);
+        float v = sum_of(idx);
+        if (PAIR) v += sum_of(idx + 4);
+        a.out[t * a.ldo + h] = __float2bfloat16_rn(v);
+      }
     }
   }
 }
@@ -538,7 +488,7 @@ void moe_layer(torch::Tensor x, torch::Tensor router, torch::Tensor gate_up, int
   const int64_t gu_rows = n_gate_up / 128 * h_kb * 128, dn_rows = h_tiles * i_kb * 128;
   for (const auto& w : {gate_up, down})
     TORCH_CHECK(w.dim() == 2 && w.size(1) == 64 && w.scalar_type() == at::kBFloat16 && w.is_contiguous() &&
-                    w.device() == x.device(),
+                    w.device() == x.device() && reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0,
                 "moe_layer: expert weights must be packed bf16 tensors [*, 64] on x's device");
   const int64_t local = gate_up.size(0) / gu_rows;
   TORCH_CHECK(local >= 1 && gate_up.size(0) == local * gu_rows && down.size(0) == local * dn_rows,
@@ -567,13 +517,6 @@ void moe_layer(torch::Tensor x, torch::Tensor router, torch::Tensor gate_up, int
   a.act = reinterpret_cast<__nv_bfloat16*>(base + head);
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
   a.ldo = T > 1 ? out.stride(0) : H;
-  const uint32_t gu_box[4] = {64, 8, kMfKb, 1}, dn_box[4] = {64, 16, kMfKb, 1};
-  const uint64_t gu_dims[4] = {64, 128, (uint64_t)h_kb, (uint64_t)(local * (n_gate_up / 128))};
-  const uint64_t gu_str[3] = {128, 128 * 128, (uint64_t)h_kb * 128 * 128};
-  const uint64_t dn_dims[4] = {64, 128, (uint64_t)i_kb, (uint64_t)(local * h_tiles)};
-  const uint64_t dn_str[3] = {128, 128 * 128, (uint64_t)i_kb * 128 * 128};
-  const CUtensorMap tg = tma_bf16(gate_up.data_ptr(), 4, gu_dims, gu_str, gu_box);
-  const CUtensorMap td = tma_bf16(down.data_ptr(), 4, dn_dims, dn_str, dn_box);
   auto stream = at::cuda::getCurrentCUDAStream();
   const __nv_bfloat16* rp = reinterpret_cast<const __nv_bfloat16*>(router.data_ptr());
   const dim3 rg((unsigned)E), rb(kMfRouterThreads);
@@ -581,13 +524,14 @@ void moe_layer(torch::Tensor x, torch::Tensor router, torch::Tensor gate_up, int
   else if (T <= 4) launch_pdl(moe_router_kernel<4>, rg, rb, 0, stream, rp, a, logits, a.counters);
   else if (T <= 8) launch_pdl(moe_router_kernel<8>, rg, rb, 0, stream, rp, a, logits, a.counters);
   else launch_pdl(moe_router_kernel<16>, rg, rb, 0, stream, rp, a, logits, a.counters);
-  const int ng = T <= 8 ? 1 : 2;
-  auto kernel = ng == 1 ? moe_few_kernel<1> : moe_few_kernel<2>;
-  const size_t smem = 1024 + (size_t)kMfStages * kMfStage + (size_t)kMfRed * kMfWarps * ng * 128 * 4 + sizeof(MfShared);
-  B200_REQUIRE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  auto kernel = T <= 4 ? moe_few_kernel<1, true> : T <= 8 ? moe_few_kernel<1, false> : moe_few_kernel<2, false>;
   const int64_t units = std::min<int64_t>(T * k, local) * (I / 8) + (H + 15) / 16;
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(units, sms)), dim3(kMfThreads), smem, stream, tg, td, a);
+  const size_t smem = T <= 8 ? sizeof(MfShared<1>) : sizeof(MfShared<2>);
+  B200_REQUIRE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(units, 2 * sms)), dim3(kMfThreads), smem, stream,
+             reinterpret_cast<const __nv_bfloat16*>(gate_up.data_ptr()),
+             reinterpret_cast<const __nv_bfloat16*>(down.data_ptr()), a);
 }
 
 int64_t moe_layer_error(bool reset) {
