@@ -255,6 +255,9 @@ class EngineConfig:
                  valid cache is read instead of the checkpoint, otherwise it is written
     step_timeout_s  watchdog: a forward step running longer fails the requests it holds
                  (their streams end with an error) and marks the engine stalled (0 = off)
+    moe_fused    MoE layers of steps with at most 16 rows (decode) through the two-kernel layer (ops.moe_layer)
+                 instead of router, permutation, grouped GEMMs and combine; activations then
+                 stay unrounded between the products, so logits differ in their last bits
     quantize     "" or "q4_k_m": quantise a bf16 checkpoint's projections to 4-bit blocks while
                  loading (GPU only; the counterpart of loading an HF model in 4 bits)
     """
@@ -284,6 +287,7 @@ class EngineConfig:
     num_layers_override: int = 0
     spec_ngram: int = 0
     spec_mtp: bool = False
+    moe_fused: bool = False
     shard_cache: str = ""
     step_timeout_s: float = 600.0
     quantize: str = ""

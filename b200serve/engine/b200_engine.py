@@ -175,6 +175,8 @@ class B200Engine(BaseEngine):
         runner = ModelRunner(mc, self.weights, self.kv, comm=self.comm, device=dev, max_batch=cfgE.max_batch,
                              kv_boundary=kv_b, boundary_layers=nb, kv_window=kv_w, window_tokens=rw,
                              max_seq=cfgE.max_seq, use_graphs=cfgE.cuda_graphs)
+        if cfgE.moe_fused and runner.decoder.moe is not None and dev.type == "cuda":
+            runner.decoder.moe.use_fused()
         if tp > 1:
             from b200serve.parallel.worker import BroadcastRunner
             runner = BroadcastRunner(runner, self.comm)
@@ -476,6 +478,29 @@ class B200Engine(BaseEngine):
             if r.embedding is None:
                 raise RuntimeError("embedding failed: " + str(self._error or "engine error"))
         return [r.embedding for r in reqs], [len(r.tokens) for r in reqs]
+
+    def score(self, prompts, timeout: float = 600.0):
+        """Log probabilities of given tokens: each prompt (text, or a list of token ids, of at most max_seq - 1
+        tokens) goes through the model once in the scheduler loop. Returns one dict per prompt with ``tokens``,
+        and ``logprobs`` and ``entropy`` (nats) of tokens[1:] given what precedes them."""
+        self.load()
+        if self.world > 1:
+            raise NotImplementedError("scoring runs on a single-rank engine")
+        self.start_loop()
+        reqs = []
+        for p in prompts:
+            ids = self.tokenizer.encode(p, add_special_tokens=False) if isinstance(p, str) else [int(t) for t in p]
+            if any(not 0 <= t < self.model_cfg.vocab_size for t in ids):
+                raise ValueError(f"scoring: token ids must lie in [0, {self.model_cfg.vocab_size})")
+            reqs.append(self.scheduler.add_scoring(Request(prompt=ids, params=SamplingParams(max_tokens=1))))
+        with self._wake:
+            self._wake.notify_all()
+        for r in reqs:
+            if not r.done_event.wait(timeout):
+                raise TimeoutError("scoring request did not finish")
+            if r.scores is None:
+                raise RuntimeError("scoring failed: " + str(self._error or "engine error"))
+        return [{"tokens": list(r.tokens), "logprobs": r.scores[0], "entropy": r.scores[1]} for r in reqs]
 
     # ------------------------------------------------------------ BaseEngine
     def _fit_prompt(self, messages, max_tokens, enable_thinking, tools):

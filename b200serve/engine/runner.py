@@ -373,6 +373,24 @@ class ModelRunner:
         self.last_prenorm, self.last_cu = (self.decoder.prenorm, cu) if fb.keep_prenorm else (None, None)
         return out
 
+    def score(self, hidden: torch.Tensor, tokens: torch.Tensor):
+        """(log probability, entropy) [n] fp32 of ``tokens`` as continuations of the final-normed hidden rows
+        ``hidden`` [n, H]. A bf16 LM head is multiplied and summed up in one kernel; a quantised one goes
+        through its logits, 512 rows at a time."""
+        if self.comm.world > 1:
+            raise NotImplementedError("scoring runs on a single-rank engine")
+        w, cap = self.decoder.w.lm_head, float(self.cfg.final_softcap or 0.0)
+        if isinstance(w, (torch.Tensor, ops.PackedWeight)):
+            return ops.linear_logprobs(hidden, w, tokens, softcap=cap)
+        parts = []
+        for i in range(0, hidden.shape[0], 512):
+            logits = ops.linear(hidden[i:i + 512], w, epilogue=ops.EPI_F32)
+            if cap:
+                ops.softcap_(logits, cap)
+            r = ops.token_logprobs(logits, tokens[i:i + 512])
+            parts.append((r.logprob, r.entropy))
+        return tuple(torch.cat(p) for p in zip(*parts))
+
     def _multimodal(self, fb, seqs, cu):
         """Images in this step (vision-language models): image rows take the vision tower's
         embeddings and the DeepStack features, and RoPE uses the three-dimensional positions

@@ -36,6 +36,7 @@ class SamplingParams:
     dry_base: float = 1.75
     dry_allowed_length: int = 2
     dry_penalty_last_n: int = -1     # -1 = whole sequence, 0 = off
+    logprobs: int = -1               # N >= 0: report log probabilities, with N alternatives (0..32) per token
 
     @property
     def greedy(self) -> bool:
@@ -63,7 +64,8 @@ class SamplingParams:
                  repeat_last_n=int(d.get("repeat_last_n", 64)), seed=d.get("seed"),
                  dry_multiplier=float(d.get("dry_multiplier", 0.0) or 0.0), dry_base=float(d.get("dry_base", 1.75)),
                  dry_allowed_length=int(d.get("dry_allowed_length", 2)),
-                 dry_penalty_last_n=int(d.get("dry_penalty_last_n", -1)))
+                 dry_penalty_last_n=int(d.get("dry_penalty_last_n", -1)),
+                 logprobs=int(d["logprobs"]) if d.get("logprobs") is not None else -1)
         if max_tokens:
             sp.max_tokens = int(max_tokens)
         stop = d.get("stop")

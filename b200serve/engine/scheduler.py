@@ -26,8 +26,10 @@ from dataclasses import dataclass, field
 
 import torch
 
+from b200serve import ops
 from b200serve.engine.kv_cache import BLOCK, BlockAllocator
 from b200serve.engine.sampler import SamplingParams, sample
+from b200serve.ops import MAX_TOP_LOGPROBS
 
 _ids = itertools.count()
 
@@ -73,6 +75,9 @@ class Request:
     state_slot: int = -1             # recurrent-state slot (hybrid models) while running
     telemetry: object = None         # TelemetryCapture: per-token forward frames (eager steps)
     embedding: list = None           # embedding requests: the mean-pooled final hidden state
+    score: bool = False              # scoring requests (add_scoring): no generation
+    scores: tuple = None             # their (log probabilities, entropies) of tokens[1:], nats
+    logprobs: list = field(default_factory=list)   # params.logprobs >= 0: one dict per output token
     mtp_draft: int = None            # MTP head's guess for the token after tokens[-1]
     mm: object = None                # models.qwen_vl.MMInput: images of a vision-language prompt
     done_event: threading.Event = field(default_factory=threading.Event)
@@ -120,6 +125,8 @@ class Scheduler:
             raise ValueError("empty prompt")
         if len(req.tokens) >= self.max_seq:
             raise ValueError(f"prompt of {len(req.tokens)} tokens exceeds max_seq {self.max_seq}")
+        if req.params.logprobs > MAX_TOP_LOGPROBS:
+            raise ValueError(f"logprobs of {req.params.logprobs} alternatives: at most {MAX_TOP_LOGPROBS}")
         if req.params.seed is not None:
             req.seed = int(req.params.seed)
         else:
@@ -142,13 +149,18 @@ class Scheduler:
             self.embed_waiting.append(req)
         return req
 
+    def add_scoring(self, req: Request) -> Request:
+        """Queue a token sequence whose tokens' log probabilities are wanted (no generation)."""
+        req.score = True
+        return self.add_embedding(req)
+
     def has_work(self) -> bool:
         return bool(self.waiting or self.running or self.embed_waiting)
 
     def _embed_step(self) -> int:
-        """One prefill of queued embedding inputs (up to ``prefill_chunk`` tokens; hybrid models one
+        """One prefill of queued embedding and scoring inputs (up to ``prefill_chunk`` tokens; hybrid models one
         input at a time, since they share the scratch state slot). Pages are borrowed for the
-        forward and returned right after; the outputs are mean-pooled per input."""
+        forward and returned right after; the outputs are mean-pooled, or scored, per input."""
         with self.lock:
             batch, total = [], 0
             for r in list(self.embed_waiting):
@@ -175,7 +187,13 @@ class Scheduler:
             off = 0
             for (r, table) in held:
                 n = len(r.tokens)
-                r.embedding = hid[off:off + n].float().mean(0).cpu().tolist()
+                if r.score:
+                    r.scores = ([], [])
+                    if n > 1:
+                        nxt = torch.as_tensor(r.tokens[1:], dtype=torch.long).to(hid.device)
+                        r.scores = tuple(t.tolist() for t in self.runner.score(hid[off:off + n - 1], nxt))
+                else:
+                    r.embedding = hid[off:off + n].float().mean(0).cpu().tolist()
                 off += n
                 r.state, r.finish_reason = "finished", "stop"
                 r.finish_time = time.perf_counter()
@@ -297,8 +315,8 @@ class Scheduler:
         waits for admission and the runner supports it (single rank, CUDA graphs)."""
         r = self.runner
         return (getattr(r, "use_graphs", False) and hasattr(r, "pipeline_step")
-                and not self.waiting and all(q.params.greedy and q.params.plain and q.telemetry is None
-                                             and q.mm is None for q in batch))
+                and not self.waiting and all(q.params.greedy and q.params.plain and q.params.logprobs < 0
+                                             and q.telemetry is None and q.mm is None for q in batch))
 
     def _pipelined_decode(self, batch) -> int:
         """Decode ``batch`` until it changes, keeping one step in flight: step N runs on the
@@ -397,13 +415,13 @@ class Scheduler:
         slots = [r.blocks[p // BLOCK] * BLOCK + p % BLOCK for r, p in zip(batch, real)]
         lens = [p + 1 for p in real]
         pos = [p + (r.mm.delta if r.mm is not None else 0) for r, p in zip(batch, real)]   # RoPE positions
-        greedy = all(r.params.greedy and r.params.plain for r in batch)
+        greedy = all(r.params.greedy and r.params.plain and r.params.logprobs < 0 for r in batch)
         watch = [(i, r.telemetry) for i, r in enumerate(batch) if r.telemetry is not None]
         kw = {"telemetry": watch} if watch else {}
         logits, toks = self.runner.decode(ids, pos, slots, [r.blocks for r in batch], lens,
                                           greedy=greedy and not watch, state_slots=[r.state_slot for r in batch], **kw)
         if toks is None:
-            toks = self._sample(logits, batch)
+            toks = self._sample_scored(logits, batch)
         toks = toks.tolist()
         for i, cap in watch:
             cap.finish_token(logits[i], toks[i])
@@ -455,7 +473,7 @@ class Scheduler:
         commits = [(i, r, r.num_computed, n) for i, (r, n) in enumerate(reqs) if seqs[i]["prenorm"]]
         for r, n in reqs:
             r.num_computed += n
-        toks = self._sample(logits, sample_reqs).tolist() if sample_reqs else []
+        toks = self._sample_scored(logits, sample_reqs).tolist() if sample_reqs else []
         for j, (r, t) in enumerate(zip(sample_reqs, toks)):
             if r.telemetry is not None:
                 r.telemetry.finish_token(logits[j], t)
@@ -492,10 +510,11 @@ class Scheduler:
 
     # ------------------------------------------------------------ speculative decoding
     def _mtp_ok(self, r: Request) -> bool:
-        return self.spec_mtp and r.params.greedy and r.params.plain and r.telemetry is None
+        return (self.spec_mtp and r.params.greedy and r.params.plain and r.params.logprobs < 0
+                and r.telemetry is None)
 
     def _spec_ok(self, r: Request) -> bool:
-        if not (r.params.greedy and r.params.plain and r.telemetry is None):
+        if not (r.params.greedy and r.params.plain and r.params.logprobs < 0 and r.telemetry is None):
             return False
         if self.spec_mtp:
             return True          # even without a draft: the verify path keeps the head's K/V complete
@@ -577,7 +596,7 @@ class Scheduler:
                 plain_reqs.append(r)
             row += n
         if plain_reqs:
-            toks = self._sample(logits[plain_rows], plain_reqs).tolist()
+            toks = self._sample_scored(logits[plain_rows], plain_reqs).tolist()
             spec += [(r, [t]) for r, t in zip(plain_reqs, toks)]
         took = {}
         for r, new in spec:
@@ -594,6 +613,25 @@ class Scheduler:
         # MTP: rows 0..(tokens taken - 1) of each verify segment are now committed positions
         self._mtp_commit([(si, 0, r, start, took.get(id(r), 0)) for si, r, start in commits])
         return accepted
+
+    def _sample_scored(self, logits, reqs) -> torch.Tensor:
+        """``_sample``, and for requests with ``params.logprobs`` >= 0 a record of the token's log probability, rank,
+        entropy and alternatives under the model's own distribution (before penalties and temperature)."""
+        want = [i for i, r in enumerate(reqs) if r.params.logprobs >= 0]
+        if not want:
+            return self._sample(logits, reqs)
+        rows = logits if len(want) == len(reqs) else logits[want]
+        if rows is logits and not all(r.params.plain for r in reqs):
+            rows = logits.clone()                    # the sampler applies penalties in place
+        toks = self._sample(logits, reqs)
+        picked = toks if len(want) == len(reqs) else toks[want]
+        lp = ops.token_logprobs(rows, picked, top=max(reqs[i].params.logprobs for i in want))
+        fields = [picked.tolist()] + [t.tolist() for t in lp]
+        for i, (tok, p, rank, ent, ids, ps) in zip(want, zip(*fields)):
+            n = reqs[i].params.logprobs
+            reqs[i].logprobs.append({"token": tok, "logprob": p, "rank": rank, "entropy": ent,
+                                     "top": [(t, v) for t, v in zip(ids[:n], ps[:n]) if t >= 0]})
+        return toks
 
     def _sample(self, logits, reqs) -> torch.Tensor:
         """``logits`` covers the whole vocabulary (the runner gathers tensor-parallel shards)."""

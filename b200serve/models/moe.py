@@ -81,6 +81,8 @@ class MoEBlock:
         self.comm = comm
         self.per = cfg.num_experts // weights.ep_size
         self.e0 = weights.ep_rank * self.per
+        self.fused_rows = 0              # steps of at most this many rows take ops.moe_layer (use_fused)
+        self.routers = {}
         self.packed = {}
         if torch.device(device).type == "cuda":
             for i, lw in enumerate(weights.layers):
@@ -90,12 +92,24 @@ class MoEBlock:
                 lw.experts_gate_up = lw.experts_down = None
             torch.cuda.empty_cache()
 
+    def use_fused(self):
+        """Steps of few rows go through ops.moe_layer from now on (EngineConfig.moe_fused). It reads the router row by
+        row, so the tile-packed one gets a plain copy (E x H)."""
+        for i, lw in enumerate(self.w.layers):
+            r = lw.router
+            self.routers[i] = r.unpacked().contiguous() if isinstance(r, ops.PackedWeight) else r
+        self.fused_rows = ops.MOE_LAYER_MAX_ROWS
+
     def _cuda(self, layer, x, fused_reduce=False):
         cfg = self.cfg
         lw = self.w.layers[layer]
         T, H = x.shape
         k = cfg.experts_per_tok
         E = self.per
+        if T <= self.fused_rows and not fused_reduce:
+            gu, n_gu, dn, n_dn = self.packed[layer]
+            return ops.moe_layer(x, self.routers[layer], gu, n_gu, dn, n_dn, k, renormalize=cfg.norm_topk_prob,
+                                 first_expert=self.e0)
         e = ops.ext()
         logits = ops.linear(x, lw.router, epilogue=ops.EPI_F32)
         wts, ids = topk_softmax(logits, k, cfg.norm_topk_prob)
