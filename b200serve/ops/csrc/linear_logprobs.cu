@@ -15,7 +15,7 @@
 //
 // Sums over H. The tensor cores cut the bits that do not fit when they add to an fp32 accumulator, so
 // the error of one long sum grows with H and has a sign: 5.5e-6 of the result's norm at H = 4096, five
-// times a rounded fp32 sum's. So only 512 elements are summed up in TMEM; the epilogue adds these
+// times a rounded fp32 sum's. So only 256 or 512 elements are summed up in TMEM; the epilogue adds these
 // parts to the 128 sums that each of its threads keeps in registers, rounding to nearest. The two TMEM
 // buffers alternate between parts, and the MMAs run on under the epilogue.
 //
@@ -31,79 +31,95 @@
 
 namespace b200 {
 
-constexpr int kLlBM = 128, kLlBN = 256, kLlBK = 64, kLlStages = 4, kLlThreads = 384;
+constexpr int kLlBM = 128, kLlBN = 256, kLlBK = 64, kLlMaxStages = 12, kLlThreads = 384;
 // registers per thread: at launch, of the producer's and the MMA issuer's warpgroup, of the epilogue's two
 constexpr int kLlRegs = 168, kLlRegsLow = 56, kLlRegsHigh = 224;
 static_assert(128 * kLlRegsLow + 256 * kLlRegsHigh == kLlThreads * kLlRegs, "the split must use what the block has");
 constexpr int kLlCols = kLlBN / 2;       // columns of an epilogue thread = of a slice
-constexpr int kLlPart = 8;               // 64-element blocks of H summed up in TMEM
-constexpr int kLlA = kLlBM * kLlBK * 2, kLlW = kLlBN * kLlBK * 2, kLlStage = kLlA + kLlW;
-constexpr size_t kLlSmem = 1024 + (size_t)kLlStages * kLlStage + 256;
+constexpr int kLlA = kLlBM * kLlBK * 2;  // a full tile of x; the MMA reads this much from a stage's start
+constexpr int kLlRing = 196608;          // bytes of all stages
+// The last stages' x windows may reach past the ring (into memory whose contents do not matter).
+constexpr size_t kLlSmem = 1024 + kLlRing + kLlA + 512;
 constexpr float kLlMasked = -1e30f;      // columns past the vocabulary: e^(x - m) is 0, products stay finite
 constexpr int64_t kLlRows = 8192;        // rows per pass: bounds the partial results (16 bytes per row and slice)
 
 static __device__ int g_ll_err;          // first error code of the bounded waits, one word per device
 
-// Work units: every row tile with `main_tiles` vocabulary tiles of 256 columns, in whole waves over
-// the SMs, then with `tail_tiles` of tail_n columns for the rest, so that the last wave is short.
+// Work units: row tiles x vocabulary tiles of tile_n columns, the row tiles of one vocabulary tile in a row.
 struct LlArgs {
-  int T, V, kb_total, m_tiles, main_tiles, tail_tiles, tail_n;
+  int T, V, kb_total, m_tiles, v_tiles, tile_n;
+  // A stage holds x_rows rows of x (128, or with one row tile just T rounded up to 16) and then tile_n of
+  // w. The MMA always takes 128 rows of x: with fewer, the others are w's bytes, and their results go nowhere.
+  int x_rows, stages, stage_bytes;
+  int part_kb;                           // 64-element blocks of H summed up in TMEM
   int packed;                            // w: tile-packed [n_tile][k_block][128][64], else plain [V, H]
-  float softcap;
+  float softcap, inv_softcap;
   TokenIds tokens;
-  int slices;                            // of 128 columns in the main part, of tail_n after it
-  float4* part;                          // [slices][T] (m, s, t, the token's logit where the slice has it)
+  int per_tile;                          // slices of up to 128 columns in a tile: 1 or 2
+  float4* part;                          // [v_tiles * per_tile][T] (m, s, t, the token's logit where the slice has it)
+};
+
+// TMA maps of w with boxes of 16, 32, 48, ... 128 rows: a tile of a packed weight takes one box per 128-row
+// weight tile that it touches. Plain weights take a tile in one box (map 0).
+struct LlMaps {
+  CUtensorMap m[8];
 };
 
 struct LlUnit {
-  int m0, v0, n, slice;                  // first row, first column, columns, first slice
+  int m0, v0, v_tile;                    // first row, first column
 };
 
 __device__ __forceinline__ LlUnit ll_unit(const LlArgs& a, int u) {
   LlUnit x;
-  const int v = u / a.m_tiles;           // the row tiles of one vocabulary tile follow one another
-  x.m0 = (u - v * a.m_tiles) * kLlBM;
-  if (v < a.main_tiles) {
-    x.v0 = v * kLlBN;
-    x.n = kLlBN;
-    x.slice = 2 * v;
-  } else {
-    const int per = a.tail_n > kLlCols ? 2 : 1;
-    x.v0 = a.main_tiles * kLlBN + (v - a.main_tiles) * a.tail_n;
-    x.n = a.tail_n;
-    x.slice = 2 * a.main_tiles + (v - a.main_tiles) * per;
-  }
+  x.v_tile = u / a.m_tiles;
+  x.m0 = (u - x.v_tile * a.m_tiles) * kLlBM;
+  x.v0 = x.v_tile * a.tile_n;
   return x;
+}
+
+// ex2 in program order: the compiler would otherwise start many of a row's 128 exponentials at once and spill
+__device__ __forceinline__ float ex2_in_order(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// tanh(y) = 1 - 2 / (1 + e^2y), off by 2^-22 at most; near zero, where that is not small beside the
+// value, the Taylor series to y^9 (the next term is below 2^-27 of y for |y| < 1/4)
+__device__ __forceinline__ float ll_tanh(float y) {
+  const float y2 = y * y;
+  const float p = y * fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(y * 2.8853900817779268f)));
+  return y2 < 0.0625f ? p : fmaf(-2.f, r, 1.f);
 }
 
 template <bool CAP>
 __global__ void __launch_bounds__(kLlThreads, 1)
-    linear_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
-                           const __grid_constant__ CUtensorMap tm_tail, const LlArgs a) {
+    linear_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ LlMaps tm_w,
+                           const LlArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* s_x = smem;
-  uint8_t* s_w = smem + kLlStages * kLlA;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kLlStages * kLlStage);
-  uint64_t* empty = full + kLlStages;
-  uint64_t* tfull = empty + kLlStages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kLlRing + kLlA);
+  uint64_t* empty = full + kLlMaxStages;
+  uint64_t* tfull = empty + kLlMaxStages;
   uint64_t* tempty = tfull + 2;
   uint64_t* mma_done = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int units = a.m_tiles * (a.main_tiles + a.tail_tiles);
+  const int units = a.m_tiles * a.v_tiles;
   int* err = &g_ll_err;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kLlStages; ++s) { tc::mbar_init(&full[s], 1); tc::mbar_init(&empty[s], 1); }
+    for (int s = 0; s < a.stages; ++s) { tc::mbar_init(&full[s], 1); tc::mbar_init(&empty[s], 1); }
     for (int i = 0; i < 2; ++i) { tc::mbar_init(&tfull[i], 1); tc::mbar_init(&tempty[i], 8); }
     tc::mbar_init(mma_done, 1);
     *abort_flag = 0;
     tc::fence_barrier_init();
     tc::fence_proxy_async_smem();
     tc::prefetch_tmap(&tm_x);
-    tc::prefetch_tmap(&tm_w);
+    for (int i = 0; i < (a.packed ? 8 : 1); ++i) tc::prefetch_tmap(&tm_w.m[i]);
   }
   __syncwarp();
   if (warp == 1) {
@@ -126,41 +142,46 @@ __global__ void __launch_bounds__(kLlThreads, 1)
       uint32_t phase = 0;
       for (int u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {
         const LlUnit x = ll_unit(a, u);
-        const CUtensorMap* map = x.n == kLlBN ? &tm_w : &tm_tail;
-        const int box = min(x.n, 128);                     // rows per box; never across a 128-row weight tile
         for (int kb = 0; kb < a.kb_total; ++kb) {
           if (!tc::mbar_wait_bounded(&empty[stage], phase ^ 1, abort_flag, err, 11)) break;
-          tc::mbar_arrive_expect_tx(&full[stage], kLlA + x.n * kLlBK * 2);
-          tc::tma_load_2d(s_x + stage * kLlA, &tm_x, &full[stage], kb * kLlBK, x.m0, pol_x);
-          for (int r = 0; r < x.n; r += box) {
-            const int v = x.v0 + r;
-            const int y = a.packed ? ((v >> 7) * a.kb_total + kb) * 128 + (v & 127) : v;
-            tc::tma_load_2d(s_w + stage * kLlW + r * 128, map, &full[stage], a.packed ? 0 : kb * kLlBK, y, pol_w);
+          uint8_t* dst = smem + stage * a.stage_bytes;
+          tc::mbar_arrive_expect_tx(&full[stage], a.stage_bytes);
+          tc::tma_load_2d(dst, &tm_x, &full[stage], kb * kLlBK, x.m0, pol_x);
+          dst += a.x_rows * 128;
+          if (!a.packed) {
+            tc::tma_load_2d(dst, &tm_w.m[0], &full[stage], kb * kLlBK, x.v0, pol_w);
+          } else {
+            for (int r = 0; r < a.tile_n;) {               // all of it in multiples of 16 rows
+              const int v = x.v0 + r, rows = min(128 - (v & 127), a.tile_n - r);
+              tc::tma_load_2d(dst + r * 128, &tm_w.m[rows / 16 - 1], &full[stage], 0,
+                              ((v >> 7) * a.kb_total + kb) * 128 + (v & 127), pol_w);
+              r += rows;
+            }
           }
-          if (++stage == kLlStages) { stage = 0; phase ^= 1; }
+          if (++stage == a.stages) { stage = 0; phase ^= 1; }
         }
       }
     }
     if (warp == 1 && lane == 0) {
       // ---------------- MMA issuer ----------------
+      const uint32_t idesc = tc::idesc_bf16_f32(kLlBM, a.tile_n);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       for (int u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {
-        const uint32_t idesc = tc::idesc_bf16_f32(kLlBM, ll_unit(a, u).n);
-        for (int k0 = 0; k0 < a.kb_total; k0 += kLlPart) {
+        for (int k0 = 0; k0 < a.kb_total; k0 += a.part_kb) {
           if (!tc::mbar_wait_bounded(&tempty[acc], acc_phase ^ 1, abort_flag, err, 12)) break;
           tc::tc_fence_after();
           const uint32_t d = tmem_base + acc * kLlBN;
-          const int kn = min(kLlPart, a.kb_total - k0);
+          const int kn = min(a.part_kb, a.kb_total - k0);
           for (int kb = 0; kb < kn; ++kb) {
             if (!tc::mbar_wait_bounded(&full[stage], phase, abort_flag, err, 13)) break;
             tc::tc_fence_after();
-            const uint64_t da = tc::sw128_kmajor_desc(tc::smem_u32(s_x + stage * kLlA));
-            const uint64_t db = tc::sw128_kmajor_desc(tc::smem_u32(s_w + stage * kLlW));
+            const uint32_t at = tc::smem_u32(smem + stage * a.stage_bytes);
+            const uint64_t da = tc::sw128_kmajor_desc(at), db = tc::sw128_kmajor_desc(at + a.x_rows * 128);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) tc::mma_bf16(d, da + 2 * kk, db + 2 * kk, idesc, (kb | kk) ? 1u : 0u);
             tc::mma_commit(&empty[stage]);
-            if (++stage == kLlStages) { stage = 0; phase ^= 1; }
+            if (++stage == a.stages) { stage = 0; phase ^= 1; }
           }
           tc::mma_commit(&tfull[acc]);
           acc ^= 1;
@@ -183,10 +204,12 @@ __global__ void __launch_bounds__(kLlThreads, 1)
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
       const LlUnit x = ll_unit(a, u);
       const int row = x.m0 + quad * 32 + lane;
-      const int cols = min(x.n - half * kLlCols, kLlCols); // <= 0: this half of a narrow tile has none
+      const int cols = min(a.tile_n - half * kLlCols, kLlCols); // <= 0: this half of a narrow tile has none
       float v[kLlCols];
+#pragma unroll
+      for (int j = 0; j < kLlCols; ++j) v[j] = 0.f;
       bool live = true;
-      for (int k0 = 0; k0 < a.kb_total; k0 += kLlPart) {
+      for (int k0 = 0; k0 < a.kb_total; k0 += a.part_kb) {
         live = __all_sync(0xffffffffu, tc::mbar_wait_bounded(&tfull[acc], acc_phase, abort_flag, err, 14));
         if (!live) break;
         tc::tc_fence_after();
@@ -196,7 +219,7 @@ __global__ void __launch_bounds__(kLlThreads, 1)
           float r[16];                                     // columns past a narrow tile: masked below
           tc::tmem_ld16(t_row + c, r);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[c + j] = k0 == 0 ? r[j] : v[c + j] + r[j];
+          for (int j = 0; j < 16; ++j) v[c + j] += r[j];
         }
         tc::tc_fence_before();
         __syncwarp();
@@ -210,7 +233,7 @@ __global__ void __launch_bounds__(kLlThreads, 1)
       const int in = min(cols, a.V - c0);
       if constexpr (CAP) {
 #pragma unroll
-        for (int j = 0; j < kLlCols; ++j) v[j] = a.softcap * tanhf(v[j] / a.softcap);
+        for (int j = 0; j < kLlCols; ++j) v[j] = a.softcap * ll_tanh(v[j] * a.inv_softcap);
       }
       if (in < kLlCols) {
 #pragma unroll
@@ -231,13 +254,13 @@ __global__ void __launch_bounds__(kLlThreads, 1)
 #pragma unroll
       for (int j = 0; j < kLlCols; ++j) {
         const float d = v[j] - m[0];
-        const float e = ex2(d * L2E);
+        const float e = ex2_in_order(d * L2E);
         s[j & 3] += e;
         t[j & 3] = fmaf(e, fmaxf(d, kLlMasked), t[j & 3]); // a logit of -inf: 0 * -1e30
       }
       const float ss = (s[0] + s[1]) + (s[2] + s[3]), tt = (t[0] + t[1]) + (t[2] + t[3]);
       if (row < a.T)
-        a.part[(size_t)(x.slice + half) * a.T + row] =
+        a.part[(size_t)(x.v_tile * a.per_tile + half) * a.T + row] =
             in > 0 ? make_float4(ss == ss ? m[0] : INFINITY, ss, tt, xt) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
     }
   }
@@ -255,7 +278,8 @@ __global__ void __launch_bounds__(kLlThreads, 1)
   }
 }
 
-// 256 threads per CTA on R rows, neighbouring threads on neighbouring rows
+// 256 threads per CTA on R rows, neighbouring threads on neighbouring rows. A thread takes its slices eight at
+// a time: one maximum for the eight and the running sum, so the chain of rescalings is short.
 constexpr int kLlRowThreads = 256;
 template <int R>
 __global__ void __launch_bounds__(kLlRowThreads) linear_logprob_rows_kernel(const LlArgs a, float* __restrict__ logprob,
@@ -265,34 +289,47 @@ __global__ void __launch_bounds__(kLlRowThreads) linear_logprob_rows_kernel(cons
   pdl_wait();
   pdl_trigger();
   const int r = threadIdx.x % R, g = threadIdx.x / R;
-  const int row = blockIdx.x * R + r;
+  const int row = blockIdx.x * R + r, S = a.v_tiles * a.per_tile;
   RowStat acc{-INFINITY, 0.f, 0.f};
   if (row < a.T) {
-#pragma unroll 8
-    for (int i = g; i < a.slices; i += G) {
-      const float4 p = __ldcg(a.part + (size_t)i * a.T + row);
-      stat_merge(acc, RowStat{p.x, p.y, p.z});
+    for (int i0 = g; i0 < S; i0 += 8 * G) {
+      float4 p[8];
+      float M = acc.m;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = i0 + j * G;
+        p[j] = i < S ? __ldcg(a.part + (size_t)i * a.T + row) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        M = fmaxf(M, p[j].x);
+      }
+      if (M == -INFINITY) continue;                    // nothing yet
+      float d = fmaxf(acc.m - M, kLlMasked), e = __expf(d), s = e * acc.s, t = e * (acc.t + d * acc.s);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        d = fmaxf(p[j].x - M, kLlMasked);              // an empty slice: e = 0
+        e = __expf(d);
+        s += e * p[j].y;
+        t += e * (p[j].z + d * p[j].y);
+      }
+      acc = RowStat{M, s, t};
     }
   }
   st[g][r] = acc;
   __syncthreads();
-  if constexpr (R == 1) {
-    if (threadIdx.x >= 32) return;
-    acc = st[threadIdx.x][0];
-    for (int i = threadIdx.x + 32; i < G; i += 32) stat_merge(acc, st[i][0]);
-    acc = stat_warp_merge(acc);
-    if (threadIdx.x != 0) return;
-  } else {
-    if (g != 0 || row >= a.T) return;
-    for (int i = 1; i < G; ++i) stat_merge(acc, st[i][r]);
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) {
+    if (g < o) {
+      stat_merge(acc, st[g + o][r]);
+      st[g][r] = acc;
+    }
+    __syncthreads();
   }
+  if (g != 0 || row >= a.T) return;
   const bool ok = stat_valid(acc);
   const int tok = token_id(a.tokens, row, a.V);
   float xt = NAN;
   if (tok >= 0) {
-    const int tail = tok - a.main_tiles * kLlBN;         // its column in the narrow tiles
-    const int slice = tail < 0 ? tok / kLlCols : 2 * a.main_tiles + tail / min(a.tail_n, kLlCols);
-    xt = __ldcg(&a.part[(size_t)slice * a.T + row].w);
+    const int v_tile = tok / a.tile_n, half = (tok - v_tile * a.tile_n) / kLlCols;
+    xt = __ldcg(&a.part[(size_t)(v_tile * a.per_tile + half) * a.T + row].w);
   }
   logprob[row] = ok ? (xt - acc.m) - logf(acc.s) : NAN;
   entropy[row] = ok ? stat_entropy(acc) : NAN;
@@ -341,38 +378,46 @@ std::vector<torch::Tensor> linear_logprobs(torch::Tensor x, torch::Tensor w, int
     LlArgs a{};
     a.T = (int)std::min(kLlRows, T - t0); a.V = (int)V; a.kb_total = kb; a.packed = packed;
     a.m_tiles = (a.T + kLlBM - 1) / kLlBM;
-    // whole waves of 256-column tiles; the columns that are left go to tiles of the width whose
-    // waves take the least time (16 more columns stand for what a tile costs at any width)
-    const int64_t all = (V + kLlBN - 1) / kLlBN, waves = a.m_tiles * all / sms;
-    a.main_tiles = (int)std::min(V / kLlBN, waves * sms / a.m_tiles);
-    const int64_t rest = V - (int64_t)a.main_tiles * kLlBN;
+    // columns per tile: of the multiples of 16 the one whose waves take the least time. 32 more columns stand
+    // for what a tile costs at any width: the rows of x, and the start of its sums.
     int64_t best = INT64_MAX;
-    a.tail_n = kLlBN;
-    for (int n = kLlBN; n >= 16 && rest > 0; n /= 2) {
-      const int64_t cost = (a.m_tiles * ((rest + n - 1) / n) + sms - 1) / sms * (n + 16);
-      if (cost < best) { best = cost; a.tail_n = n; }
+    for (int n = kLlBN; n >= 32; n -= 16) {
+      const int64_t cost = ((int64_t)a.m_tiles * ((V + n - 1) / n) + sms - 1) / sms * (n + 32);
+      if (cost < best) { best = cost; a.tile_n = n; }
     }
-    a.tail_tiles = (int)((rest + a.tail_n - 1) / a.tail_n);
-    a.slices = 2 * a.main_tiles + a.tail_tiles * (a.tail_n > kLlCols ? 2 : 1);
+    a.v_tiles = (int)((V + a.tile_n - 1) / a.tile_n);
+    a.per_tile = a.tile_n > kLlCols ? 2 : 1;
+    const int64_t slices = (int64_t)a.v_tiles * a.per_tile;
+    a.inv_softcap = softcap > 0.0 ? (float)(1.0 / softcap) : 0.f;
+    // 256 elements per part where the read of w is the bound, else 512 (the epilogue's additions then stay under the
+    // MMAs: 2048 rows of H = 4096 take 2.10 ms instead of 2.29)
+    a.part_kb = a.m_tiles == 1 ? 4 : 8;
     a.softcap = (float)softcap;
     const bool is64 = tokens.scalar_type() == at::kLong;
     a.tokens = TokenIds{static_cast<const char*>(tokens.data_ptr()) + t0 * (is64 ? 8 : 4), is64};
-    const int64_t need = (int64_t)a.slices * a.T * 4;
+    const int64_t need = slices * a.T * 4;
     if (!part.defined() || part.numel() < need) part = torch::empty({need}, logprob.options());
     a.part = reinterpret_cast<float4*>(part.data_ptr());
     const void* xp = static_cast<const __nv_bfloat16*>(x.data_ptr()) + t0 * ldx;
     const uint64_t xd[2] = {(uint64_t)H, (uint64_t)a.T}, xs[1] = {(uint64_t)ldx * 2};
-    const uint32_t xb[2] = {64, kLlBM};
+    a.x_rows = a.m_tiles > 1 ? kLlBM : (a.T + 15) / 16 * 16;
+    a.stage_bytes = (a.x_rows + a.tile_n) * 128;
+    a.stages = std::min(kLlMaxStages, kLlRing / a.stage_bytes);
+    const uint32_t xb[2] = {64, (uint32_t)a.x_rows};
     const uint64_t wd[2] = {packed ? 64ull : (uint64_t)H, (uint64_t)w.size(0)}, ws[1] = {(packed ? 64 : H) * 2ull};
-    const uint32_t wb[2] = {64, 128}, tb[2] = {64, (uint32_t)std::min(a.tail_n, 128)};
-    const CUtensorMap tx = tma_bf16(xp, 2, xd, xs, xb), tw = tma_bf16(w.data_ptr(), 2, wd, ws, wb),
-                      tt = tma_bf16(w.data_ptr(), 2, wd, ws, tb);
-    const int64_t units = (int64_t)a.m_tiles * (a.main_tiles + a.tail_tiles);
+    const CUtensorMap tx = tma_bf16(xp, 2, xd, xs, xb);
+    LlMaps tw;
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t wb[2] = {64, (uint32_t)(packed ? 16 * (i + 1) : a.tile_n)};
+      tw.m[i] = i == 0 || packed ? tma_bf16(w.data_ptr(), 2, wd, ws, wb) : tw.m[0];
+    }
+    const int64_t units = (int64_t)a.m_tiles * a.v_tiles;
     const unsigned grid = (unsigned)std::min<int64_t>(units, sms);
-    launch_pdl(kernel, dim3(grid), dim3(kLlThreads), kLlSmem, stream, tx, tw, tt, a);
+    launch_pdl(kernel, dim3(grid), dim3(kLlThreads), kLlSmem, stream, tx, tw, a);
     float* lp = logprob.data_ptr<float>() + t0;
     float* en = entropy.data_ptr<float>() + t0;
-    if (a.T >= 8)
+    // one row per CTA while that is at most four CTAs an SM, then eight (whole 128-byte lines of the partial results)
+    if (a.T > 4 * sms)
       launch_pdl(linear_logprob_rows_kernel<8>, dim3((unsigned)((a.T + 7) / 8)), dim3(kLlRowThreads), 0, stream, a, lp,
                  en);
     else

@@ -7,15 +7,16 @@
 //     work on one read. Bound by HBM (4 or 2 bytes a logit) once there are rows for every SM.
 //   * logprob_rows: one CTA per row joins the slices' statistics and merges their sorted lists.
 //
-// Selection. The `top`-th largest of the 256 per-thread maxima is at most the `top`-th largest logit
-// of the slice. One warp finds a value with at least `top` and at most top + 12 maxima at or above
-// it by descending the bits of the (order-preserving) values; only those threads look at their 32
-// or 64 logits again and push what reaches the value into a list, which is ranked by counting. The
-// rank goes by a 64-bit key (value bits, then the complement of the id), so keys are unique and
-// "ties: the lowest id" is the key order. Where too many maxima are equal for any value to do,
-// the same search runs over the keys of the maxima instead. Either way the list is bounded by
-// (top + 12) threads' logits, for any data. The row kernel selects among the slices' lists
-// the same way, from the lists' heads.
+// Selection. With the slice's logits in 32 groups (a lane of every warp), the `top`-th largest group
+// maximum is at most the `top`-th largest logit, and for logits in no particular order few more than
+// `top` reach it (31 on average for 20 of 8192). One warp finds a value just below it by descending the
+// bits of the order-preserving values under votes; only threads whose maximum reaches the value look
+// at their logits again and push what reaches it into a list, which is ranked by counting. The rank
+// goes by a 64-bit key (value bits, then the complement of the id), so keys are unique and "ties: the
+// lowest id" is the key order. Where more than the list holds reach the value (equal or sorted
+// logits), the threshold is the `top`-th largest of the 256 per-thread largest keys instead: at most
+// `top` threads' logits lie at or above it, for any data. The row kernel selects among the slices'
+// lists the same way, from the lists' heads.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -25,7 +26,6 @@
 namespace b200 {
 
 constexpr int kLpThreads = 256;
-constexpr int kLpSlack = 12;             // accepted surplus of per-thread maxima above the threshold
 
 // order-preserving bits of a logit; 0 for anything that is never an alternative (-inf, NaN)
 __device__ __forceinline__ uint32_t logit_bits(float x) {
@@ -50,31 +50,11 @@ struct LpArgs {
   unsigned long long* keys;              // [B][S][top] descending, 0 = none
 };
 
-// The largest value whose bits, from `bit` down to 0, can be set with at least `top` of the warp's N * 32
-// keys at or above it; stops early at top + kLpSlack. Returns the number of keys at or above it.
-template <typename K, int N>
-__device__ __forceinline__ int key_threshold(const K (&k)[N], int top, int bit, K& thr) {
-  int have = N * 32;
-  for (; bit >= 0; --bit) {
-    const K c = thr | (K(1) << bit);
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) n += k[i] >= c;
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (n >= top) {
-      thr = c;
-      have = n;
-      if (n <= top + kLpSlack) break;
-    }
-  }
-  return have;
-}
-
 // T = float or __nv_bfloat16; U 16-byte pieces per thread
 template <typename T, int U>
 __global__ void __launch_bounds__(kLpThreads, U == 8 && sizeof(T) == 2 ? 2 : 4) logprob_slices_kernel(const LpArgs a) {
   constexpr int VEC = 16 / (int)sizeof(T), NV = U * VEC, SLICE = kLpThreads * NV, WARPS = kLpThreads / 32;
-  constexpr int CAP = (kMaxTop + kLpSlack) * NV;
+  constexpr int CAP = kMaxTop * NV;
   __shared__ float red[WARPS][4];
   __shared__ uint32_t tmax[kLpThreads];
   __shared__ unsigned long long tkey[kLpThreads];
@@ -133,21 +113,23 @@ __global__ void __launch_bounds__(kLpThreads, U == 8 && sizeof(T) == 2 ? 2 : 4) 
 
   // ---- threshold (the other warps go on with the sums)
   if (a.top > 0 && warp == WARPS - 1) {
-    uint32_t k[WARPS], any = 0, all = 0xffffffffu;
+    uint32_t k = 0;
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) {
-      k[i] = tmax[i * 32 + lane];
-      any |= k[i];
-      all &= k[i];
-    }
-    any = __reduce_or_sync(0xffffffffu, any);
-    all = __reduce_and_sync(0xffffffffu, all);
+    for (int i = 0; i < WARPS; ++i) k = max(k, tmax[i * 32 + lane]);
+    const uint32_t any = __reduce_or_sync(0xffffffffu, k), all = __reduce_and_sync(0xffffffffu, k);
     // the bits above the highest one in which the maxima differ are common to all of them
-    const int bit = 31 - __clz((any & ~all) | 1u);
+    int bit = 31 - __clz((any & ~all) | 1u);
     uint32_t thr = bit == 31 ? 0u : all >> (bit + 1) << (bit + 1);
-    const int n = key_threshold<uint32_t>(k, a.top, bit, thr);
-    // 0: fewer than `top` threads hold a logit above -inf; all logits are candidates
-    if (lane == 0) thr_s = thr == 0u ? -3.402823466e38f : n <= a.top + kLpSlack ? logit_of_bits(thr) : NAN;
+    for (; bit >= 0; --bit) {
+      const uint32_t c = thr | (1u << bit);
+      const int n = __popc(__ballot_sync(0xffffffffu, k >= c));
+      if (n >= a.top) {
+        thr = c;
+        if (n <= a.top + 1) break;
+      }
+    }
+    // 0: fewer than `top` groups hold a logit above -inf; all logits are candidates
+    if (lane == 0) thr_s = thr == 0u ? -3.402823466e38f : logit_of_bits(thr);
   }
 
   // ---- sums and the count of logits that rank before the token
@@ -186,17 +168,17 @@ __global__ void __launch_bounds__(kLpThreads, U == 8 && sizeof(T) == 2 ? 2 : 4) 
 
   // ---- candidates (the order of the list does not matter)
   const float thr = thr_s;
-  if (thr == thr) {
-    if (tm >= thr) {
+  if (tm >= thr) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (v[i] >= thr) {
-          const int p = atomicAdd(&count_s, 1);
-          if (p < CAP) list[p] = logit_key(v[i], id_of(i));
-        }
-    }
-  } else {
-    // too many equal maxima: a thread's largest key is its maximum at the lowest id that holds it
+    for (int i = 0; i < NV; ++i)
+      if (v[i] >= thr) {
+        const int p = atomicAdd(&count_s, 1);
+        if (p < CAP) list[p] = logit_key(v[i], id_of(i));
+      }
+  }
+  __syncthreads();
+  if (count_s > CAP) {
+    // a thread's largest key is its maximum at the lowest id that holds it
     int at = 0;
 #pragma unroll
     for (int i = NV - 1; i >= 0; --i)
@@ -204,13 +186,11 @@ __global__ void __launch_bounds__(kLpThreads, U == 8 && sizeof(T) == 2 ? 2 : 4) 
     const unsigned long long mine = logit_key(tm, at);
     tkey[tid] = mine;
     __syncthreads();
-    if (warp == 0) {
-      unsigned long long k[WARPS], key = 0;
-#pragma unroll
-      for (int i = 0; i < WARPS; ++i) k[i] = tkey[i * 32 + lane];
-      key_threshold<unsigned long long>(k, a.top, 63, key);
-      if (lane == 0) thr_key_s = key;
-    }
+    if (tid == 0) { count_s = 0; thr_key_s = 1ull; }   // 1: fewer than `top` threads hold a logit: all logits
+    __syncthreads();
+    int above = 0;
+    for (int j = 0; j < kLpThreads; ++j) above += tkey[j] > mine;
+    if (mine && above == a.top - 1) thr_key_s = mine;
     __syncthreads();
     const unsigned long long key = thr_key_s;
     if (mine >= key) {
@@ -223,8 +203,8 @@ __global__ void __launch_bounds__(kLpThreads, U == 8 && sizeof(T) == 2 ? 2 : 4) 
         }
       }
     }
+    __syncthreads();
   }
-  __syncthreads();
   const int n = min(count_s, CAP);
   unsigned long long* out = a.keys + (row * a.S + slice) * a.top;
   for (int i = tid; i < n; i += kLpThreads) {
@@ -373,8 +353,9 @@ std::vector<torch::Tensor> token_logprobs(torch::Tensor logits, torch::Tensor to
     else launch_slices<float, 8>(a, (int)B, stream);
   }
   const size_t smem = (size_t)a.S * top * 16;           // at most 129 slices of 32 keys, twice
-  B200_REQUIRE_CUDA(cudaFuncSetAttribute(bf ? logprob_rows_kernel<__nv_bfloat16> : logprob_rows_kernel<float>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024));
+  if (smem > 40 * 1024)
+    B200_REQUIRE_CUDA(cudaFuncSetAttribute(bf ? logprob_rows_kernel<__nv_bfloat16> : logprob_rows_kernel<float>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024));
   if (bf) launch_pdl(logprob_rows_kernel<__nv_bfloat16>, dim3((unsigned)B), dim3(kLpRowThreads), smem, stream, a, o);
   else launch_pdl(logprob_rows_kernel<float>, dim3((unsigned)B), dim3(kLpRowThreads), smem, stream, a, o);
   return res;
