@@ -9,6 +9,10 @@
 //   instead of 512 of logits.
 //   linear_logprob_rows: joins the slices of every row.
 //
+// With more than 128 rows two CTAs of a cluster work on one tile of 256 rows (cta_group::2): each
+// loads its 128 rows of x and half of the tile's columns of w, so an SM reads 32 KB for 64 elements of H
+// instead of 48 KB. One CTA per tile reads 64 bytes a clock there, which is what the L2 gives an SM.
+//
 // Roles (384 threads): warp 0 TMA producer, warp 1 MMA issuer, warps 4..11 epilogue (two per TMEM
 // lane quarter, 128 of the tile's columns each). The epilogue's sums need more than the 168
 // registers that 384 threads can have: the first warpgroup gives up 112 of its own to the other two.
@@ -47,7 +51,7 @@ static __device__ int g_ll_err;          // first error code of the bounded wait
 
 // Work units: row tiles x vocabulary tiles of tile_n columns, the row tiles of one vocabulary tile in a row.
 struct LlArgs {
-  int T, V, kb_total, m_tiles, v_tiles, tile_n;
+  int T, V, kb_total, m_tiles, v_tiles, tile_m, tile_n;
   // A stage holds x_rows rows of x (128, or with one row tile just T rounded up to 16) and then tile_n of
   // w. The MMA always takes 128 rows of x: with fewer, the others are w's bytes, and their results go nowhere.
   int x_rows, stages, stage_bytes;
@@ -72,7 +76,7 @@ struct LlUnit {
 __device__ __forceinline__ LlUnit ll_unit(const LlArgs& a, int u) {
   LlUnit x;
   x.v_tile = u / a.m_tiles;
-  x.m0 = (u - x.v_tile * a.m_tiles) * kLlBM;
+  x.m0 = (u - x.v_tile * a.m_tiles) * a.tile_m;
   x.v0 = x.v_tile * a.tile_n;
   return x;
 }
@@ -94,7 +98,66 @@ __device__ __forceinline__ float ll_tanh(float y) {
   return y2 < 0.0625f ? p : fmaf(-2.f, r, 1.f);
 }
 
-template <bool CAP>
+// ---- two-CTA forms of the tensor-core instructions (CG = 2), one-CTA forms otherwise
+template <int CG>
+__device__ __forceinline__ void ll_tma(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, uint64_t hint) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(tc::smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "l"(hint)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(tc::smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "l"(hint)
+        : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void ll_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    tc::mma_bf16(d, da, db, idesc, accumulate);
+}
+// arrives on `bar` (of both CTAs) once the MMAs issued so far are complete
+template <int CG>
+__device__ __forceinline__ void ll_commit(uint64_t* bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            tc::smem_u32(bar)), "h"((unsigned short)3)
+        : "memory");
+  else
+    tc::mma_commit(bar);
+}
+template <int CG>
+__device__ __forceinline__ void ll_tmem_alloc(uint32_t* slot) {
+  if constexpr (CG == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(slot)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tc::tmem_alloc(slot, 512);
+    tc::tmem_relinquish();
+  }
+}
+template <int CG>
+__device__ __forceinline__ void ll_tmem_free(uint32_t base) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(512) : "memory");
+  else
+    tc::tmem_dealloc(base, 512);
+}
+
+// CG: CTAs per tile. Rank 0 of a pair issues the MMAs of both; the barriers that it waits on are its own.
+template <bool CAP, int CG>
 __global__ void __launch_bounds__(kLlThreads, 1)
     linear_logprobs_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ LlMaps tm_w,
                            const LlArgs a) {
@@ -109,11 +172,12 @@ __global__ void __launch_bounds__(kLlThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = a.m_tiles * a.v_tiles;
+  const int rank = CG == 2 ? (int)tc::cluster_ctarank() : 0, first = blockIdx.x / CG, step = gridDim.x / CG;
   int* err = &g_ll_err;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.stages; ++s) { tc::mbar_init(&full[s], 1); tc::mbar_init(&empty[s], 1); }
-    for (int i = 0; i < 2; ++i) { tc::mbar_init(&tfull[i], 1); tc::mbar_init(&tempty[i], 8); }
+    for (int i = 0; i < 2; ++i) { tc::mbar_init(&tfull[i], 1); tc::mbar_init(&tempty[i], 8 * CG); }
     tc::mbar_init(mma_done, 1);
     *abort_flag = 0;
     tc::fence_barrier_init();
@@ -123,11 +187,11 @@ __global__ void __launch_bounds__(kLlThreads, 1)
   }
   __syncwarp();
   if (warp == 1) {
-    tc::tmem_alloc(tmem_slot, 512);
-    tc::tmem_relinquish();
+    ll_tmem_alloc<CG>(tmem_slot);
   }
   tc::tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) tc::cluster_sync();               // the peer's barriers are ready
   tc::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();
@@ -140,21 +204,24 @@ __global__ void __launch_bounds__(kLlThreads, 1)
       const uint64_t pol_w = tc::policy_evict_first(), pol_x = tc::policy_evict_last();
       int stage = 0;
       uint32_t phase = 0;
-      for (int u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {
+      for (int u = first; u < units && !*abort_flag; u += step) {
         const LlUnit x = ll_unit(a, u);
         for (int kb = 0; kb < a.kb_total; ++kb) {
           if (!tc::mbar_wait_bounded(&empty[stage], phase ^ 1, abort_flag, err, 11)) break;
           uint8_t* dst = smem + stage * a.stage_bytes;
-          tc::mbar_arrive_expect_tx(&full[stage], a.stage_bytes);
-          tc::tma_load_2d(dst, &tm_x, &full[stage], kb * kLlBK, x.m0, pol_x);
+          uint32_t bar = tc::smem_u32(&full[stage]);
+          if constexpr (CG == 2) bar = tc::map_shared_rank(bar, 0);
+          if (rank == 0) tc::mbar_arrive_expect_tx(&full[stage], CG * a.stage_bytes);
+          ll_tma<CG>(dst, &tm_x, bar, kb * kLlBK, x.m0 + rank * kLlBM, pol_x);
           dst += a.x_rows * 128;
+          const int w_rows = a.tile_n / CG, v0 = x.v0 + rank * w_rows;
           if (!a.packed) {
-            tc::tma_load_2d(dst, &tm_w.m[0], &full[stage], kb * kLlBK, x.v0, pol_w);
+            ll_tma<CG>(dst, &tm_w.m[0], bar, kb * kLlBK, v0, pol_w);
           } else {
-            for (int r = 0; r < a.tile_n;) {               // all of it in multiples of 16 rows
-              const int v = x.v0 + r, rows = min(128 - (v & 127), a.tile_n - r);
-              tc::tma_load_2d(dst + r * 128, &tm_w.m[rows / 16 - 1], &full[stage], 0,
-                              ((v >> 7) * a.kb_total + kb) * 128 + (v & 127), pol_w);
+            for (int r = 0; r < w_rows;) {                 // all of it in multiples of 16 rows
+              const int v = v0 + r, rows = min(128 - (v & 127), w_rows - r);
+              ll_tma<CG>(dst + r * 128, &tm_w.m[rows / 16 - 1], bar, 0, ((v >> 7) * a.kb_total + kb) * 128 + (v & 127),
+                         pol_w);
               r += rows;
             }
           }
@@ -162,12 +229,12 @@ __global__ void __launch_bounds__(kLlThreads, 1)
         }
       }
     }
-    if (warp == 1 && lane == 0) {
+    if (warp == 1 && lane == 0 && rank == 0) {
       // ---------------- MMA issuer ----------------
-      const uint32_t idesc = tc::idesc_bf16_f32(kLlBM, a.tile_n);
+      const uint32_t idesc = tc::idesc_bf16_f32(CG * kLlBM, a.tile_n);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
-      for (int u = blockIdx.x; u < units && !*abort_flag; u += gridDim.x) {
+      for (int u = first; u < units && !*abort_flag; u += step) {
         for (int k0 = 0; k0 < a.kb_total; k0 += a.part_kb) {
           if (!tc::mbar_wait_bounded(&tempty[acc], acc_phase ^ 1, abort_flag, err, 12)) break;
           tc::tc_fence_after();
@@ -179,17 +246,17 @@ __global__ void __launch_bounds__(kLlThreads, 1)
             const uint32_t at = tc::smem_u32(smem + stage * a.stage_bytes);
             const uint64_t da = tc::sw128_kmajor_desc(at), db = tc::sw128_kmajor_desc(at + a.x_rows * 128);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) tc::mma_bf16(d, da + 2 * kk, db + 2 * kk, idesc, (kb | kk) ? 1u : 0u);
-            tc::mma_commit(&empty[stage]);
+            for (int kk = 0; kk < 4; ++kk) ll_mma<CG>(d, da + 2 * kk, db + 2 * kk, idesc, (kb | kk) ? 1u : 0u);
+            ll_commit<CG>(&empty[stage]);
             if (++stage == a.stages) { stage = 0; phase ^= 1; }
           }
-          tc::mma_commit(&tfull[acc]);
+          ll_commit<CG>(&tfull[acc]);
           acc ^= 1;
           if (acc == 0) acc_phase ^= 1;
         }
       }
       // no tcgen05.mma may still be running when TMEM is released below
-      tc::mma_commit(mma_done);
+      ll_commit<CG>(mma_done);
       volatile int never = 0;
       tc::mbar_wait_bounded(mma_done, 0, &never, err, 15);
     }
@@ -201,9 +268,14 @@ __global__ void __launch_bounds__(kLlThreads, 1)
     const float L2E = 1.4426950408889634f;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    uint32_t drained[2] = {tc::smem_u32(&tempty[0]), tc::smem_u32(&tempty[1])};
+    if constexpr (CG == 2) {
+      drained[0] = tc::map_shared_rank(drained[0], 0);
+      drained[1] = tc::map_shared_rank(drained[1], 0);
+    }
+    for (int u = first; u < units; u += step) {
       const LlUnit x = ll_unit(a, u);
-      const int row = x.m0 + quad * 32 + lane;
+      const int row = x.m0 + rank * kLlBM + quad * 32 + lane;
       const int cols = min(a.tile_n - half * kLlCols, kLlCols); // <= 0: this half of a narrow tile has none
       float v[kLlCols];
 #pragma unroll
@@ -223,7 +295,13 @@ __global__ void __launch_bounds__(kLlThreads, 1)
         }
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&tempty[acc]);
+        if (lane == 0) {
+          if constexpr (CG == 2)
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc ? drained[1] : drained[0])
+                         : "memory");
+          else
+            tc::mbar_arrive(&tempty[acc]);
+        }
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
@@ -272,9 +350,16 @@ __global__ void __launch_bounds__(kLlThreads, 1)
     while (globaltimer_ns() < until) {
     }
   }
+  // no CTA of a pair leaves while the other may still signal its barriers or multiply from its memory
+  if constexpr (CG == 2) {
+    volatile int never = 0;
+    if (rank == 1 && threadIdx.x == 32) tc::mbar_wait_bounded(mma_done, 0, &never, err, 16);
+    __syncwarp();
+    tc::cluster_sync();
+  }
   if (warp == 1) {
     tc::tc_fence_after();
-    tc::tmem_dealloc(tmem_base, 512);
+    ll_tmem_free<CG>(tmem_base);
   }
 }
 
@@ -368,21 +453,25 @@ std::vector<torch::Tensor> linear_logprobs(torch::Tensor x, torch::Tensor w, int
 
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   auto stream = at::cuda::getCurrentCUDAStream();
-  auto kernel = softcap > 0.0 ? linear_logprobs_kernel<true> : linear_logprobs_kernel<false>;
-  cudaFuncAttributes attr;
-  B200_REQUIRE_CUDA(cudaFuncGetAttributes(&attr, kernel));
-  B200_REQUIRE(attr.numRegs == kLlRegs, "linear_logprobs: the register split does not fit this build");
-  B200_REQUIRE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLlSmem));
   torch::Tensor part;
   for (int64_t t0 = 0; t0 < T; t0 += kLlRows) {
     LlArgs a{};
     a.T = (int)std::min(kLlRows, T - t0); a.V = (int)V; a.kb_total = kb; a.packed = packed;
-    a.m_tiles = (a.T + kLlBM - 1) / kLlBM;
+    const int cg = a.T > kLlBM ? 2 : 1;
+    a.tile_m = cg * kLlBM;
+    a.m_tiles = (a.T + a.tile_m - 1) / a.tile_m;
+    auto kernel = cg == 2 ? (softcap > 0.0 ? linear_logprobs_kernel<true, 2> : linear_logprobs_kernel<false, 2>)
+                          : (softcap > 0.0 ? linear_logprobs_kernel<true, 1> : linear_logprobs_kernel<false, 1>);
+    cudaFuncAttributes attr;
+    B200_REQUIRE_CUDA(cudaFuncGetAttributes(&attr, kernel));
+    B200_REQUIRE(attr.numRegs == kLlRegs, "linear_logprobs: the register split does not fit this build");
+    B200_REQUIRE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLlSmem));
+    const int slots = sms / cg;                          // CTAs, or pairs of them, at a time
     // columns per tile: of the multiples of 16 the one whose waves take the least time. 32 more columns stand
     // for what a tile costs at any width: the rows of x, and the start of its sums.
     int64_t best = INT64_MAX;
-    for (int n = kLlBN; n >= 32; n -= 16) {
-      const int64_t cost = ((int64_t)a.m_tiles * ((V + n - 1) / n) + sms - 1) / sms * (n + 32);
+    for (int n = kLlBN; n >= 32; n -= 16 * cg) {
+      const int64_t cost = ((int64_t)a.m_tiles * ((V + n - 1) / n) + slots - 1) / slots * (n + 32);
       if (cost < best) { best = cost; a.tile_n = n; }
     }
     a.v_tiles = (int)((V + a.tile_n - 1) / a.tile_n);
@@ -391,7 +480,7 @@ std::vector<torch::Tensor> linear_logprobs(torch::Tensor x, torch::Tensor w, int
     a.inv_softcap = softcap > 0.0 ? (float)(1.0 / softcap) : 0.f;
     // 256 elements per part where the read of w is the bound, else 512 (the epilogue's additions then stay under the
     // MMAs: 2048 rows of H = 4096 take 2.10 ms instead of 2.29)
-    a.part_kb = a.m_tiles == 1 ? 4 : 8;
+    a.part_kb = cg == 1 ? 4 : 8;
     a.softcap = (float)softcap;
     const bool is64 = tokens.scalar_type() == at::kLong;
     a.tokens = TokenIds{static_cast<const char*>(tokens.data_ptr()) + t0 * (is64 ? 8 : 4), is64};
@@ -400,20 +489,23 @@ std::vector<torch::Tensor> linear_logprobs(torch::Tensor x, torch::Tensor w, int
     a.part = reinterpret_cast<float4*>(part.data_ptr());
     const void* xp = static_cast<const __nv_bfloat16*>(x.data_ptr()) + t0 * ldx;
     const uint64_t xd[2] = {(uint64_t)H, (uint64_t)a.T}, xs[1] = {(uint64_t)ldx * 2};
-    a.x_rows = a.m_tiles > 1 ? kLlBM : (a.T + 15) / 16 * 16;
-    a.stage_bytes = (a.x_rows + a.tile_n) * 128;
+    a.x_rows = cg == 2 ? kLlBM : (a.T + 15) / 16 * 16;
+    a.stage_bytes = (a.x_rows + a.tile_n / cg) * 128;
     a.stages = std::min(kLlMaxStages, kLlRing / a.stage_bytes);
     const uint32_t xb[2] = {64, (uint32_t)a.x_rows};
     const uint64_t wd[2] = {packed ? 64ull : (uint64_t)H, (uint64_t)w.size(0)}, ws[1] = {(packed ? 64 : H) * 2ull};
     const CUtensorMap tx = tma_bf16(xp, 2, xd, xs, xb);
     LlMaps tw;
     for (int i = 0; i < 8; ++i) {
-      const uint32_t wb[2] = {64, (uint32_t)(packed ? 16 * (i + 1) : a.tile_n)};
+      const uint32_t wb[2] = {64, (uint32_t)(packed ? 16 * (i + 1) : a.tile_n / cg)};
       tw.m[i] = i == 0 || packed ? tma_bf16(w.data_ptr(), 2, wd, ws, wb) : tw.m[0];
     }
     const int64_t units = (int64_t)a.m_tiles * a.v_tiles;
-    const unsigned grid = (unsigned)std::min<int64_t>(units, sms);
-    launch_pdl(kernel, dim3(grid), dim3(kLlThreads), kLlSmem, stream, tx, tw, a);
+    const unsigned grid = (unsigned)(std::min<int64_t>(units, slots) * cg);
+    if (cg == 2)
+      launch_pdl_cluster(kernel, dim3(grid), dim3(kLlThreads), kLlSmem, stream, 2, tx, tw, a);
+    else
+      launch_pdl(kernel, dim3(grid), dim3(kLlThreads), kLlSmem, stream, tx, tw, a);
     float* lp = logprob.data_ptr<float>() + t0;
     float* en = entropy.data_ptr<float>() + t0;
     // one row per CTA while that is at most four CTAs an SM, then eight (whole 128-byte lines of the partial results)
