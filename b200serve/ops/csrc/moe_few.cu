@@ -21,7 +21,7 @@
 // agree on), so a warp's load covers eight whole 64-byte pieces. The tensor pipe is a few percent
 // busy; tcgen05 tiles of 128 weight rows would only coarsen the units that balance the SMs. TMA
 // into shared memory was slower here: boxes of 8 rows and the waits on 24 stages took 0.25 us per
-// 8 KB and SM, 218 us where this takes 169 (16 rows, 128 experts of 768, top 8, 2048 wide).
+// 8 KB and SM, 218 us where this takes 151 (16 rows, 128 experts of 768, top 8, 2048 wide).
 //
 // Numerics: fp32 accumulation; the routing weight is folded into the activation in fp32, and the
 // activation is kept as the sum of two bf16 (high part and remainder, 16 bits of mantissa), so
@@ -365,14 +365,19 @@ __global__ void __launch_bounds__(kMfThreads, 2)
 
     int sl = up ? 0 : warp / dn_chunks, ks = warp - sl * dn_chunks;
     for (int c = warp; c < chunks; c += kMfWarps) {
-      fill(n + 1);
-      // the oldest chunk has landed once at most ahead - 1 groups are on the way
-      if (ahead >= 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-      else if (ahead == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else asm volatile("cp.async.wait_group 0;" ::: "memory");
       uint4 w[2][2][2];
+      bool have_w = false;
+      auto take_w = [&]() {                                // starts further copies, waits for the oldest chunk
+        fill(n + 1);
+        // it has landed once at most ahead - 1 groups are on the way
+        if (ahead >= 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+        else if (ahead == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i >> 2][i >> 1 & 1][i & 1] = sh.ring[out_slot][i][tid];
+        for (int i = 0; i < 8; ++i) w[i >> 2][i >> 1 & 1][i & 1] = sh.ring[out_slot][i][tid];
+        have_w = true;
+      };
+      // activations first: their way from L2 passes under the copies and the wait
       const int k0 = ks * 128 + 8 * t4;
       if (up) {
 #pragma unroll
@@ -383,6 +388,7 @@ __global__ void __launch_bounds__(kMfThreads, 2)
           for (int i = 0; i < 4; ++i)
             b[i] = xrow[q] != nullptr && k0 + 32 * i < a.H ? *reinterpret_cast<const uint4*>(xrow[q] + k0 + 32 * i)
                                                            : zero;
+          if (!have_w) take_w();
 #pragma unroll
           for (int i = 0; i < 4; ++i) mma_piece(acc[q][i & 1], w[i >> 1][i & 1][0], w[i >> 1][i & 1][1], b[i]);
         }
@@ -403,6 +409,7 @@ __global__ void __launch_bounds__(kMfThreads, 2)
             for (int i = 0; i < 4; ++i)
               b[j][i] = in && k0 + 32 * i < a.I ? *reinterpret_cast<const uint4*>(arow + j * act_rows * a.I + 32 * i)
                                                 : zero;
+          if (!have_w) take_w();
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
