@@ -1406,8 +1406,8 @@ def linear_logprobs(x, w, tokens, softcap=0.0):
         raise TypeError(f"linear_logprobs: w must be a tensor or a PackedWeight, got {type(w).__name__}")
     if x.shape[1] != w.shape[1]:
         raise ValueError(f"linear_logprobs: x has {x.shape[1]} columns, w {w.shape[1]}")
-    if softcap < 0:
-        raise ValueError(f"linear_logprobs: softcap must not be negative, got {softcap}")
+    if not 0 <= softcap < math.inf:
+        raise ValueError(f"linear_logprobs: softcap must be finite and not negative, got {softcap}")
     if _cuda(x, 2):
         return tuple(ext().linear_logprobs(x, w.data if packed else w, w.N if packed else 0, tokens, float(softcap)))
     logits = x.float() @ (w.unpacked() if packed else w).float().t()

@@ -4,7 +4,7 @@
 //
 // With so few rows the layer is the read of the chosen experts' weights, 6 H I bytes each, and
 // what costs besides is every wait between dependent steps. So:
-//   * moe_router: one CTA per expert row of R computes its logit for every token.
+//   * moe_router: one CTA per expert row of R and four tokens computes their logits.
 //   * moe_few: two CTAs of eight warps per SM. Every CTA repeats the tiny routing step for itself,
 //     then takes units of work from one counter: first all gate/up units (8 inner columns of one
 //     expert: 8 gate and 8 up rows), then all down units (16 output rows over every chosen
@@ -63,13 +63,13 @@ template <int TT>
 __global__ void __launch_bounds__(kMfRouterThreads) moe_router_kernel(const __nv_bfloat16* __restrict__ router, const MfArgs a,
                                                          float* __restrict__ logits, int* __restrict__ counters) {
   __shared__ float red[kMfRouterThreads / 32][TT];
-  const int e = blockIdx.x, tid = threadIdx.x;
+  const int e = blockIdx.x, tid = threadIdx.x, t0 = blockIdx.y * TT;
   const __nv_bfloat16* w = router + (size_t)e * a.H;
   bf16x8 first{};                                // a weight: does not depend on the previous kernel
   if (tid * 8 < a.H) first = *reinterpret_cast<const bf16x8*>(w + tid * 8);
   pdl_trigger();
   pdl_wait();
-  if (e == 0 && tid < 2) counters[tid] = 0;
+  if (e == 0 && t0 == 0 && tid < 2) counters[tid] = 0;
   float acc[TT];
 #pragma unroll
   for (int t = 0; t < TT; ++t) acc[t] = 0.f;
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kMfRouterThreads) moe_router_kernel(const __nv
     bf16x8 xv[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t)                 // rows past T repeat the last one: loads without branches
-      xv[t] = *reinterpret_cast<const bf16x8*>(a.x + min(t, a.T - 1) * a.ldx + i);
+      xv[t] = *reinterpret_cast<const bf16x8*>(a.x + min(t0 + t, a.T - 1) * a.ldx + i);
     float wf[8];
     unpack8(wv, wf);
 #pragma unroll
@@ -95,11 +95,11 @@ __global__ void __launch_bounds__(kMfRouterThreads) moe_router_kernel(const __nv
     if ((tid & 31) == 0) red[tid >> 5][t] = s;
   }
   __syncthreads();
-  if (tid < a.T) {
+  if (tid < TT && t0 + tid < a.T) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < kMfRouterThreads / 32; ++i) s += red[i][tid];
-    logits[(size_t)tid * a.E + e] = s;
+    logits[(size_t)(t0 + tid) * a.E + e] = s;
   }
 }
 
@@ -526,11 +526,9 @@ void moe_layer(torch::Tensor x, torch::Tensor router, torch::Tensor gate_up, int
   a.ldo = T > 1 ? out.stride(0) : H;
   auto stream = at::cuda::getCurrentCUDAStream();
   const __nv_bfloat16* rp = reinterpret_cast<const __nv_bfloat16*>(router.data_ptr());
-  const dim3 rg((unsigned)E), rb(kMfRouterThreads);
+  const dim3 rg((unsigned)E, (unsigned)((T + 3) / 4)), rb(kMfRouterThreads);
   if (T <= 1) launch_pdl(moe_router_kernel<1>, rg, rb, 0, stream, rp, a, logits, a.counters);
-  else if (T <= 4) launch_pdl(moe_router_kernel<4>, rg, rb, 0, stream, rp, a, logits, a.counters);
-  else if (T <= 8) launch_pdl(moe_router_kernel<8>, rg, rb, 0, stream, rp, a, logits, a.counters);
-  else launch_pdl(moe_router_kernel<16>, rg, rb, 0, stream, rp, a, logits, a.counters);
+  else launch_pdl(moe_router_kernel<4>, rg, rb, 0, stream, rp, a, logits, a.counters);
   auto kernel = T <= 4 ? moe_few_kernel<1, true> : T <= 8 ? moe_few_kernel<1, false> : moe_few_kernel<2, false>;
   const int64_t units = std::min<int64_t>(T * k, local) * (I / 8) + (H + 15) / 16;
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;

@@ -77,8 +77,9 @@ def test_refusals():
     h, w = torch.zeros(2, 16).bfloat16(), torch.zeros(10, 16).bfloat16()
     with pytest.raises(ValueError):
         ops.linear_logprobs(h, w[:, :8], tok)
-    with pytest.raises(ValueError):
-        ops.linear_logprobs(h, w, tok, softcap=-1.0)
+    for cap in (-1.0, INF, NAN):
+        with pytest.raises(ValueError):
+            ops.linear_logprobs(h, w, tok, softcap=cap)
     with pytest.raises(TypeError):
         ops.linear_logprobs(h, [w], tok)
     c = MoECase(T=2, H=64, E=4, k=2, inner=64)
