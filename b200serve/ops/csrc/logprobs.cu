@@ -75,11 +75,14 @@ __global__ void __launch_bounds__(kLpThreads, U == 8 && sizeof(T) == 2 ? 2 : 4) 
   const int tok = token_id(a.tokens, row, a.V);
   const float xt = tok >= 0 ? (float)x[tok] : INFINITY;
 
+  // all of the slice lies in the row (the first and the last may not)
+  const bool inside = slice * SLICE >= shift && (slice + 1) * SLICE - shift <= a.V;
+
   float v[NV];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int id0 = id_of(u * VEC);
-    if (id0 >= 0 && id0 + VEC <= a.V) {
+    if (inside || (id0 >= 0 && id0 + VEC <= a.V)) {
       const uint4 w = *reinterpret_cast<const uint4*>(x + id0);
       if constexpr (VEC == 4) {
         v[u * 4 + 0] = __uint_as_float(w.x); v[u * 4 + 1] = __uint_as_float(w.y);
@@ -169,11 +172,17 @@ __global__ void __launch_bounds__(kLpThreads, U == 8 && sizeof(T) == 2 ? 2 : 4) 
   // ---- candidates (the order of the list does not matter)
   const float thr = thr_s;
   if (tm >= thr) {
+    // a mask without branches first; the few logits in it are read again (registers have no index)
+    uint32_t hit[(NV + 31) / 32] = {};
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (v[i] >= thr) {
+      if (v[i] >= thr) hit[i / 32] |= 1u << (i % 32);
+#pragma unroll
+    for (int h = 0; h < (NV + 31) / 32; ++h)
+      for (uint32_t m = hit[h]; m; m &= m - 1u) {
+        const int id = id_of(h * 32 + __ffs(m) - 1);
         const int p = atomicAdd(&count_s, 1);
-        if (p < CAP) list[p] = logit_key(v[i], id_of(i));
+        if (p < CAP) list[p] = logit_key((float)x[id], id);
       }
   }
   __syncthreads();
