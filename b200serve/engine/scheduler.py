@@ -188,10 +188,11 @@ class Scheduler:
             for (r, table) in held:
                 n = len(r.tokens)
                 if r.score:
-                    r.scores = ([], [])
+                    scores = ([], [])                # a single token has nothing to score
                     if n > 1:
                         nxt = torch.as_tensor(r.tokens[1:], dtype=torch.long).to(hid.device)
-                        r.scores = tuple(t.tolist() for t in self.runner.score(hid[off:off + n - 1], nxt))
+                        scores = tuple(t.tolist() for t in self.runner.score(hid[off:off + n - 1], nxt))
+                    r.scores = scores                # None until then: how the caller tells a failed step
                 else:
                     r.embedding = hid[off:off + n].float().mean(0).cpu().tolist()
                 off += n

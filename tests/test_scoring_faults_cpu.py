@@ -1,0 +1,37 @@
+"""Scoring and log-probability requests that fail, or that must not be taken, through the engine (CPU)."""
+
+import pytest
+import torch
+
+from b200serve.core.config import EngineConfig
+from b200serve.engine.b200_engine import B200Engine
+from b200serve.models.config import BUILTIN
+from b200serve.models.weights import random_weights
+
+
+@pytest.fixture(scope="module")
+def engine():
+    w = random_weights(BUILTIN["tiny-qwen2"], seed=0, dtype=torch.float32)
+    eng = B200Engine(EngineConfig(model="tiny-qwen2", device="cpu", dtype="float32", cuda_graphs=False, max_seq=128,
+                                  max_batch=4), weights=w)
+    eng.load()
+    yield eng
+    eng.unload()
+
+
+def test_a_failed_score_raises(engine, monkeypatch):
+    """A runner whose score raises fails the caller, whichever of its prompts that was."""
+    real = engine.runner.score
+
+    def score(hidden, tokens):
+        if 99 in tokens.tolist():
+            raise MemoryError("no room for the partial results")
+        return real(hidden, tokens)
+
+    monkeypatch.setattr(engine.runner, "score", score)
+    for prompts in ([[1, 2, 99, 4]], [[1, 2, 3], [4, 5, 6, 7], [8, 99]]):
+        with pytest.raises(RuntimeError, match="scoring failed"):
+            engine.score(prompts, timeout=60)
+    monkeypatch.undo()
+    [ok] = engine.score([[1, 2, 3, 4]], timeout=60)          # the engine goes on
+    assert len(ok["logprobs"]) == len(ok["entropy"]) == 3
