@@ -486,13 +486,16 @@ class B200Engine(BaseEngine):
         self.load()
         if self.world > 1:
             raise NotImplementedError("scoring runs on a single-rank engine")
-        self.start_loop()
         reqs = []
-        for p in prompts:
+        for p in prompts:                            # all of them are checked before any is queued
             ids = self.tokenizer.encode(p, add_special_tokens=False) if isinstance(p, str) else [int(t) for t in p]
             if any(not 0 <= t < self.model_cfg.vocab_size for t in ids):
                 raise ValueError(f"scoring: token ids must lie in [0, {self.model_cfg.vocab_size})")
-            reqs.append(self.scheduler.add_scoring(Request(prompt=ids, params=SamplingParams(max_tokens=1))))
+            reqs.append(Request(prompt=ids, params=SamplingParams(max_tokens=1)))
+            self.scheduler.check_embedding(reqs[-1])
+        self.start_loop()
+        for r in reqs:
+            self.scheduler.add_scoring(r)
         with self._wake:
             self._wake.notify_all()
         for r in reqs:

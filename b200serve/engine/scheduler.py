@@ -141,10 +141,14 @@ class Scheduler:
     def abort(self, req: Request):
         req.aborted = True
 
-    def add_embedding(self, req: Request) -> Request:
-        """Queue a prompt whose mean-pooled final hidden state is wanted (no generation)."""
+    def check_embedding(self, req: Request):
+        """Refuses an embedding or scoring input that no step could take."""
         if not req.tokens or len(req.tokens) >= self.max_seq:
             raise ValueError(f"embedding input of {len(req.tokens)} tokens: must be 1..{self.max_seq - 1}")
+
+    def add_embedding(self, req: Request) -> Request:
+        """Queue a prompt whose mean-pooled final hidden state is wanted (no generation)."""
+        self.check_embedding(req)
         with self.lock:
             self.embed_waiting.append(req)
         return req

@@ -35,3 +35,16 @@ def test_a_failed_score_raises(engine, monkeypatch):
     monkeypatch.undo()
     [ok] = engine.score([[1, 2, 3, 4]], timeout=60)          # the engine goes on
     assert len(ok["logprobs"]) == len(ok["entropy"]) == 3
+
+
+def test_a_refused_prompt_queues_nothing(engine):
+    seen = []
+    real = engine.scheduler.add_embedding
+    engine.scheduler.add_embedding = lambda r: (seen.append(r), real(r))[1]
+    try:
+        for bad in ([1] * 128, [], [32000], [-1]):
+            with pytest.raises(ValueError):
+                engine.score([[1, 2, 3], bad], timeout=60)
+    finally:
+        del engine.scheduler.add_embedding
+    assert not seen and not engine.scheduler.embed_waiting
