@@ -145,6 +145,9 @@ class Scheduler:
         """Refuses an embedding or scoring input that no step could take."""
         if not req.tokens or len(req.tokens) >= self.max_seq:
             raise ValueError(f"embedding input of {len(req.tokens)} tokens: must be 1..{self.max_seq - 1}")
+        if len(req.tokens) > self.alloc.num_blocks * BLOCK:      # would wait for pages for good
+            raise ValueError(f"embedding input of {len(req.tokens)} tokens: the KV cache holds "
+                             f"{self.alloc.num_blocks * BLOCK}")
 
     def add_embedding(self, req: Request) -> Request:
         """Queue a prompt whose mean-pooled final hidden state is wanted (no generation)."""

@@ -48,3 +48,16 @@ def test_a_refused_prompt_queues_nothing(engine):
     finally:
         del engine.scheduler.add_embedding
     assert not seen and not engine.scheduler.embed_waiting
+
+
+def test_a_prompt_larger_than_the_cache_is_refused():
+    w = random_weights(BUILTIN["tiny-qwen2"], seed=0, dtype=torch.float32)
+    eng = B200Engine(EngineConfig(model="tiny-qwen2", device="cpu", dtype="float32", cuda_graphs=False, max_seq=128,
+                                  max_batch=1, kv_blocks=4), weights=w)
+    try:
+        with pytest.raises(ValueError, match="KV cache"):
+            eng.score([[1] * 65], timeout=3)
+        [ok] = eng.score([[1] * 64], timeout=60)
+        assert len(ok["logprobs"]) == 63
+    finally:
+        eng.unload()
