@@ -502,7 +502,7 @@ class B200Engine(BaseEngine):
             if not r.done_event.wait(timeout):
                 raise TimeoutError("scoring request did not finish")
             if r.scores is None:
-                raise RuntimeError("scoring failed: " + str(self._error or "engine error"))
+                raise RuntimeError("scoring failed: " + str(r.error or self._error or "engine error")) from r.error
         return [{"tokens": list(r.tokens), "logprobs": r.scores[0], "entropy": r.scores[1]} for r in reqs]
 
     # ------------------------------------------------------------ BaseEngine

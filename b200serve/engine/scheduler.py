@@ -77,6 +77,7 @@ class Request:
     embedding: list = None           # embedding requests: the mean-pooled final hidden state
     score: bool = False              # scoring requests (add_scoring): no generation
     scores: tuple = None             # their (log probabilities, entropies) of tokens[1:], nats
+    error: Exception = None          # why the scores could not be computed
     logprobs: list = field(default_factory=list)   # params.logprobs >= 0: one dict per output token
     mtp_draft: int = None            # MTP head's guess for the token after tokens[-1]
     mm: object = None                # models.qwen_vl.MMInput: images of a vision-language prompt
@@ -196,14 +197,17 @@ class Scheduler:
                 n = len(r.tokens)
                 if r.score:
                     scores = ([], [])                # a single token has nothing to score
-                    if n > 1:
-                        nxt = torch.as_tensor(r.tokens[1:], dtype=torch.long).to(hid.device)
-                        scores = tuple(t.tolist() for t in self.runner.score(hid[off:off + n - 1], nxt))
-                    r.scores = scores                # None until then: how the caller tells a failed step
+                    try:
+                        if n > 1:
+                            nxt = torch.as_tensor(r.tokens[1:], dtype=torch.long).to(hid.device)
+                            scores = tuple(t.tolist() for t in self.runner.score(hid[off:off + n - 1], nxt))
+                        r.scores = scores            # None until then: how the caller tells a failed step
+                    except Exception as e:           # (no room, say) concerns this request alone
+                        r.error = e
                 else:
                     r.embedding = hid[off:off + n].float().mean(0).cpu().tolist()
                 off += n
-                r.state, r.finish_reason = "finished", "stop"
+                r.state, r.finish_reason = "finished", "error" if r.error is not None else "stop"
                 r.finish_time = time.perf_counter()
         finally:
             for r, table in held:

@@ -5,6 +5,7 @@ import torch
 
 from b200serve.core.config import EngineConfig
 from b200serve.engine.b200_engine import B200Engine
+from b200serve.engine.sampler import SamplingParams
 from b200serve.models.config import BUILTIN
 from b200serve.models.weights import random_weights
 
@@ -61,3 +62,23 @@ def test_a_prompt_larger_than_the_cache_is_refused():
         assert len(ok["logprobs"]) == 63
     finally:
         eng.unload()
+
+
+def test_a_failed_score_leaves_other_requests_alone(engine, monkeypatch):
+    """A generation under way, and another scoring call of the same step, end as they would without it."""
+    def score(hidden, tokens):
+        if 99 in tokens.tolist():
+            raise MemoryError("no room for the partial results")
+        return real(hidden, tokens)
+
+    from b200serve.engine.scheduler import Request
+    real = engine.runner.score
+    prompt, params = list(range(10, 30)), SamplingParams(max_tokens=40, ignore_eos=True)
+    [want] = engine.generate([prompt], params, timeout=60)
+    monkeypatch.setattr(engine.runner, "score", score)
+    req = engine.submit(Request(prompt=prompt, params=params))
+    good = engine.scheduler.add_scoring(Request(prompt=[5, 6, 7], params=SamplingParams(max_tokens=1)))
+    with pytest.raises(RuntimeError, match="no room"):
+        engine.score([[1, 99]], timeout=60)
+    assert req.done_event.wait(60) and good.done_event.wait(60)
+    assert req.finish_reason == "length" and req.output == want.output and len(good.scores[0]) == 2
