@@ -18,6 +18,13 @@ import torch
 from b200serve import ops
 
 
+def _logprobs_count(v) -> int:
+    """``SamplingParams.logprobs`` as a count: off (-1) for None and False, no alternatives (0) for True."""
+    if v is None or isinstance(v, bool):
+        return 0 if v else -1
+    return int(v)
+
+
 @dataclass
 class SamplingParams:
     temperature: float = 0.0
@@ -37,6 +44,10 @@ class SamplingParams:
     dry_allowed_length: int = 2
     dry_penalty_last_n: int = -1     # -1 = whole sequence, 0 = off
     logprobs: int = -1               # N >= 0: report log probabilities, with N alternatives (0..32) per token
+                                     # (True: without alternatives; False: off)
+
+    def __post_init__(self):
+        self.logprobs = _logprobs_count(self.logprobs)
 
     @property
     def greedy(self) -> bool:
@@ -65,7 +76,7 @@ class SamplingParams:
                  dry_multiplier=float(d.get("dry_multiplier", 0.0) or 0.0), dry_base=float(d.get("dry_base", 1.75)),
                  dry_allowed_length=int(d.get("dry_allowed_length", 2)),
                  dry_penalty_last_n=int(d.get("dry_penalty_last_n", -1)),
-                 logprobs=int(d["logprobs"]) if d.get("logprobs") is not None else -1)
+                 logprobs=_logprobs_count(d.get("logprobs")))
         if max_tokens:
             sp.max_tokens = int(max_tokens)
         stop = d.get("stop")

@@ -82,3 +82,11 @@ def test_a_failed_score_leaves_other_requests_alone(engine, monkeypatch):
         engine.score([[1, 99]], timeout=60)
     assert req.done_event.wait(60) and good.done_event.wait(60)
     assert req.finish_reason == "length" and req.output == want.output and len(good.scores[0]) == 2
+
+
+def test_logprobs_switch_takes_truth_values():
+    for value, n in ((False, -1), (None, -1), (True, 0), (0, 0), (7, 7), (-1, -1)):
+        assert SamplingParams.from_dict({"logprobs": value}).logprobs == n
+        assert SamplingParams(logprobs=value).logprobs == n
+        assert type(SamplingParams(logprobs=value).logprobs) is int
+    assert SamplingParams.from_dict({}).logprobs == SamplingParams().logprobs == -1
