@@ -535,6 +535,8 @@ class B200Engine(BaseEngine):
                            web_tools=False, reasoning_effort=None, on_telemetry=None, sampling=None,
                            tools=None, images=None) -> str:
         self.load()
+        if sampling and "logprobs" in sampling:      # the stream carries text only: no records, and no price for them
+            sampling = {k: v for k, v in sampling.items() if k != "logprobs"}
         params = SamplingParams.from_dict(sampling, temperature=temperature,
                                           max_tokens=max_tokens if max_tokens and max_tokens > 0 else 8192)
         prompt, fit = self._fit_prompt(messages, params.max_tokens, enable_thinking, tools)

@@ -90,3 +90,15 @@ def test_logprobs_switch_takes_truth_values():
         assert SamplingParams(logprobs=value).logprobs == n
         assert type(SamplingParams(logprobs=value).logprobs) is int
     assert SamplingParams.from_dict({}).logprobs == SamplingParams().logprobs == -1
+
+
+def test_streaming_ignores_logprobs(engine, monkeypatch):
+    """A text stream returns no records, so the key neither slows its requests nor refuses them."""
+    seen = []
+    real = engine.submit
+    monkeypatch.setattr(engine, "submit", lambda r: (seen.append(r), real(r))[1])
+    msgs = [{"role": "user", "content": "hi"}]
+    want = engine.generate_streaming(msgs, 4, 0.0, sampling={"top_k": 1})
+    for value in (5, 50, True, False, "many"):
+        assert engine.generate_streaming(msgs, 4, 0.0, sampling={"top_k": 1, "logprobs": value}) == want
+    assert len(seen) == 6 and all(r.params.logprobs == -1 and r.logprobs == [] for r in seen)
