@@ -257,7 +257,9 @@ class EngineConfig:
                  (their streams end with an error) and marks the engine stalled (0 = off)
     moe_fused    MoE layers of steps with at most 16 rows (decode) through the two-kernel layer (ops.moe_layer)
                  instead of router, permutation, grouped GEMMs and combine; activations then
-                 stay unrounded between the products, so logits differ in their last bits
+                 stay unrounded between the products, so logits differ in their last bits. For one rank,
+                 and for several with comm="nccl": the fused communicator keeps its own combine
+                 kernel, and the option stays off with a warning
     quantize     "" or "q4_k_m": quantise a bf16 checkpoint's projections to 4-bit blocks while
                  loading (GPU only; the counterpart of loading an HF model in 4 bits)
     """

@@ -10,10 +10,14 @@ dense FFN uses.
 
 from __future__ import annotations
 
+import logging
+
 import torch
 
 from b200serve import ops
 from b200serve.models.weights import interleave_gate_up, pad_down, pad64
+
+_log = logging.getLogger(__name__)
 
 
 def shard_layer_moe(cfg, full, lw, ep_rank, ep_size, dtype, device):
@@ -92,13 +96,19 @@ class MoEBlock:
                 lw.experts_gate_up = lw.experts_down = None
             torch.cuda.empty_cache()
 
-    def use_fused(self):
+    def use_fused(self) -> bool:
         """Steps of few rows go through ops.moe_layer from now on (EngineConfig.moe_fused). It reads the router row by
-        row, so the tile-packed one gets a plain copy (E x H)."""
+        row, so the tile-packed one gets a plain copy (E x H). False, with a warning, where no step would take it:
+        a communicator that sums the experts' outputs inside its combine kernel takes all of them (``reduced``)."""
+        if hasattr(self.comm, "moe_combine_reduce") and getattr(self.comm, "max_tokens", 0) >= ops.MOE_LAYER_MAX_ROWS:
+            _log.warning("b200: moe_fused is off: this communicator fuses the combine of decode-sized steps with its "
+                         "sum over the ranks")
+            return False
         for i, lw in enumerate(self.w.layers):
             r = lw.router
             self.routers[i] = r.unpacked().contiguous() if isinstance(r, ops.PackedWeight) else r
         self.fused_rows = ops.MOE_LAYER_MAX_ROWS
+        return True
 
     def _cuda(self, layer, x, fused_reduce=False):
         cfg = self.cfg
