@@ -259,7 +259,8 @@ class EngineConfig:
                  instead of router, permutation, grouped GEMMs and combine; activations then
                  stay unrounded between the products, so logits differ in their last bits. For one rank,
                  and for several with comm="nccl": the fused communicator keeps its own combine
-                 kernel, and the option stays off with a warning
+                 kernel, and the option stays off with a warning, as it does for models of more than
+                 256 experts or more than 16 per token
     quantize     "" or "q4_k_m": quantise a bf16 checkpoint's projections to 4-bit blocks while
                  loading (GPU only; the counterpart of loading an HF model in 4 bits)
     """

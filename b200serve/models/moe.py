@@ -98,11 +98,17 @@ class MoEBlock:
 
     def use_fused(self) -> bool:
         """Steps of few rows go through ops.moe_layer from now on (EngineConfig.moe_fused). It reads the router row by
-        row, so the tile-packed one gets a plain copy (E x H). False, with a warning, where no step would take it:
-        a communicator that sums the experts' outputs inside its combine kernel takes all of them (``reduced``)."""
+        row, so the tile-packed one gets a plain copy (E x H). False, with a warning, where no step could take it:
+        a communicator that sums the experts' outputs inside its combine kernel takes all of them (``reduced``), and
+        models may have more experts than the layer."""
         if hasattr(self.comm, "moe_combine_reduce") and getattr(self.comm, "max_tokens", 0) >= ops.MOE_LAYER_MAX_ROWS:
             _log.warning("b200: moe_fused is off: this communicator fuses the combine of decode-sized steps with its "
                          "sum over the ranks")
+            return False
+        E, k = self.cfg.num_experts, self.cfg.experts_per_tok
+        if E > ops.MOE_LAYER_MAX_EXPERTS or k > ops.MOE_LAYER_MAX_TOP:
+            _log.warning("b200: moe_fused is off: it takes up to %d experts and %d of them per token, this model has %d "
+                         "and %d", ops.MOE_LAYER_MAX_EXPERTS, ops.MOE_LAYER_MAX_TOP, E, k)
             return False
         for i, lw in enumerate(self.w.layers):
             r = lw.router

@@ -1423,6 +1423,7 @@ def linear_logprobs_error(reset: bool = True) -> int:
 
 # ------------------------------------------------------------------ mixture of experts, few tokens
 MOE_LAYER_MAX_ROWS = 16
+MOE_LAYER_MAX_EXPERTS, MOE_LAYER_MAX_TOP = 256, 16
 
 
 def moe_layer(x, router, gate_up, n_gate_up, down, n_down, k, renormalize=True, first_expert=0, out=None):
@@ -1447,7 +1448,7 @@ def moe_layer(x, router, gate_up, n_gate_up, down, n_down, k, renormalize=True, 
     E, inner = router.shape[0], n_gate_up // 2
     gu_rows, dn_rows = n_gate_up * ((H + 63) // 64), (H + 127) // 128 * 2 * inner
     local = gate_up.shape[0] // gu_rows
-    if not (1 <= k <= min(16, E) and E <= 256):
+    if not (1 <= k <= min(MOE_LAYER_MAX_TOP, E) and E <= MOE_LAYER_MAX_EXPERTS):
         raise ValueError(f"moe_layer: 1 to 256 experts and 1 to 16 of them per token, got {E} and {k}")
     if local < 1 or gate_up.shape[0] != local * gu_rows or down.shape[0] != local * dn_rows:
         raise ValueError("moe_layer: packed expert weights have the wrong shape")

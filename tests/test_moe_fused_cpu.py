@@ -39,3 +39,12 @@ def test_fused_communicator_keeps_its_own_combine(caplog):
     with caplog.at_level(logging.WARNING):
         assert b.use_fused() is False
     assert "moe_fused is off" in caplog.text and b.routers == {} and b.fused_rows == 0
+
+
+@pytest.mark.parametrize("cfg,on", [(dict(num_experts=512), False), (dict(num_experts=256), True),
+                                    (dict(num_experts=32, experts_per_tok=17), False)])
+def test_models_past_the_layers_limits_keep_the_grouped_path(cfg, on, caplog):
+    b = _block(**cfg)
+    with caplog.at_level(logging.WARNING):
+        assert b.use_fused() is on
+    assert ("moe_fused is off" in caplog.text) != on and bool(b.routers) == on and bool(b.fused_rows) == on
