@@ -37,10 +37,11 @@ struct RowStat {
   float m, s, t;
 };
 
-// Adds slice (m, s, t) to `a`. m = -inf marks an empty slice (its s and t are 0).
+// Adds slice (m, s, t) to `a`. m = -inf marks an empty slice (its s and t are 0). The differences are bounded so
+// that a slice which does not count (all of it at the type's lowest value, say) adds e^d d s = 0, not 0 * -inf.
 __device__ __forceinline__ void stat_merge(RowStat& a, const RowStat& b) {
   const float M = fmaxf(a.m, b.m);
-  const float da = a.m - M, db = b.m - M;
+  const float da = fmaxf(a.m - M, -1e30f), db = fmaxf(b.m - M, -1e30f);
   if (a.m == -INFINITY) {
     a = b;
   } else if (b.m != -INFINITY) {
