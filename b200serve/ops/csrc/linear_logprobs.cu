@@ -44,7 +44,7 @@ constexpr int kLlA = kLlBM * kLlBK * 2;  // a full tile of x; the MMA reads this
 constexpr int kLlRing = 196608;          // bytes of all stages
 // The last stages' x windows may reach past the ring (into memory whose contents do not matter).
 constexpr size_t kLlSmem = 1024 + kLlRing + kLlA + 512;
-constexpr float kLlMasked = -1e30f;      // columns past the vocabulary: e^(x - m) is 0, products stay finite
+constexpr float kLlFloor = -1e30f;       // lower bound of x - m in products with e^(x - m) = 0, which stay 0
 constexpr int64_t kLlRows = 8192;        // rows per pass: bounds the partial results (16 bytes per row and slice)
 
 static __device__ int g_ll_err;          // first error code of the bounded waits, one word per device
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(kLlThreads, 1)
       if (in < kLlCols) {
 #pragma unroll
         for (int j = 0; j < kLlCols; ++j)
-          if (j >= in) v[j] = kLlMasked;
+          if (j >= in) v[j] = -INFINITY;                   // past the vocabulary: counts for nothing
       }
       float xt = 0.f;
       const int at = row < a.T ? token_id(a.tokens, row, a.V) - c0 : -1;
@@ -324,22 +324,22 @@ __global__ void __launch_bounds__(kLlThreads, 1)
 #pragma unroll
         for (int j = 0; j < kLlCols; ++j) xt = j == at ? v[j] : xt;
       }
-      float m[4] = {kLlMasked, kLlMasked, kLlMasked, kLlMasked};
+      float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int j = 0; j < kLlCols; ++j) m[j & 3] = fmaxf(m[j & 3], v[j]);
       m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      const float mm = m[0] == -INFINITY ? 0.f : m[0];     // nothing above -inf: all terms are 0
       float s[4] = {0.f, 0.f, 0.f, 0.f}, t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < kLlCols; ++j) {
-        const float d = v[j] - m[0];
+        const float d = v[j] - mm;
         const float e = ex2_in_order(d * L2E);
         s[j & 3] += e;
-        t[j & 3] = fmaf(e, fmaxf(d, kLlMasked), t[j & 3]); // a logit of -inf: 0 * -1e30
+        t[j & 3] = fmaf(e, fmaxf(d, kLlFloor), t[j & 3]);  // a logit of -inf: 0 * -1e30
       }
       const float ss = (s[0] + s[1]) + (s[2] + s[3]), tt = (t[0] + t[1]) + (t[2] + t[3]);
       if (row < a.T)
-        a.part[(size_t)(x.v_tile * a.per_tile + half) * a.T + row] =
-            in > 0 ? make_float4(ss == ss ? m[0] : INFINITY, ss, tt, xt) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        a.part[(size_t)(x.v_tile * a.per_tile + half) * a.T + row] = make_float4(ss == ss ? m[0] : INFINITY, ss, tt, xt);
     }
   }
   tc::tc_fence_before();
@@ -387,10 +387,10 @@ __global__ void __launch_bounds__(kLlRowThreads) linear_logprob_rows_kernel(cons
         M = fmaxf(M, p[j].x);
       }
       if (M == -INFINITY) continue;                    // nothing yet
-      float d = fmaxf(acc.m - M, kLlMasked), e = __expf(d), s = e * acc.s, t = e * (acc.t + d * acc.s);
+      float d = fmaxf(acc.m - M, kLlFloor), e = __expf(d), s = e * acc.s, t = e * (acc.t + d * acc.s);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        d = fmaxf(p[j].x - M, kLlMasked);              // an empty slice: e = 0
+        d = fmaxf(p[j].x - M, kLlFloor);               // an empty slice: e = 0
         e = __expf(d);
         s += e * p[j].y;
         t += e * (p[j].z + d * p[j].y);

@@ -1,10 +1,12 @@
 """Log-probability kernels at the edges of their inputs' range, against 64-bit references."""
 
+import math
+
 import pytest
 import torch
 
 from b200serve import ops
-from logprob_cases import check_token_logprobs
+from logprob_cases import check_token_logprobs, entropy_bound, log_s_bound
 
 pytestmark = pytest.mark.gpu
 dev = "cuda"
@@ -30,3 +32,26 @@ def test_whole_slices_at_the_lowest_value(dtype):
     x = x.to(dtype)
     tokens = torch.tensor([5, 29500, 7, 12000, 3], device=dev)
     check_token_logprobs(ops.token_logprobs(x, tokens, top=20), x, tokens, 20)
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("T", [2, 200])
+def test_logits_far_below_zero(packed, T):
+    """Every logit of a row below -1e30: what pads a tile past the vocabulary must not count. 300 and 40 tokens
+    leave the last tile part empty; the 2^100s are exact, and differ by 0 or by 2^100."""
+    for V in (300, 40):
+        x = torch.zeros(T, 64, device=dev, dtype=torch.bfloat16)
+        w = torch.zeros(V, 64, device=dev, dtype=torch.bfloat16)
+        x[:, 0], w[:, 0] = 1, -(2.0 ** 101)
+        tokens = torch.full((T,), 7, device=dev)
+        head = ops.PackedWeight(w) if packed else w
+        lp, ent = ops.linear_logprobs(x, head, tokens)
+        want = math.log(V)                               # uniform
+        assert float((lp + want).abs().max()) < log_s_bound(V) + want * 2.0 ** -22
+        assert float((ent - want).abs().max()) < entropy_bound(V)
+        w[9, 0] = -(2.0 ** 100)                          # one token takes everything
+        head = ops.PackedWeight(w) if packed else w
+        lp, ent = ops.linear_logprobs(x, head, tokens)
+        assert bool((lp == -(2.0 ** 100)).all() and (ent == 0).all())
+        tokens[:] = 9
+        assert bool((ops.linear_logprobs(x, head, tokens)[0] == 0).all())
