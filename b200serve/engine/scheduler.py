@@ -201,6 +201,9 @@ class Scheduler:
                         if n > 1:
                             nxt = torch.as_tensor(r.tokens[1:], dtype=torch.long).to(hid.device)
                             scores = tuple(t.tolist() for t in self.runner.score(hid[off:off + n - 1], nxt))
+                            code = ops.linear_logprobs_error()
+                            if code:
+                                raise RuntimeError(f"a wait inside the scoring kernel ran out (code {code})")
                         r.scores = scores            # None until then: how the caller tells a failed step
                     except Exception as e:           # (no room, say) concerns this request alone
                         r.error = e

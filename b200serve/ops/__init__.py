@@ -1417,8 +1417,9 @@ def linear_logprobs(x, w, tokens, softcap=0.0):
 
 
 def linear_logprobs_error(reset: bool = True) -> int:
-    """First error code of linear_logprobs' bounded waits on the current device (0 = none)."""
-    return int(ext().linear_logprobs_error(reset)) if extension_loaded() else 0
+    """First error code of linear_logprobs' bounded waits on the current device (0 = none), over the calls that
+    have finished. From a wait that ran out until the code is read and reset, results are NaN."""
+    return int(ext().linear_logprobs_error(0 if reset else -1)) if extension_loaded() else 0
 
 
 # ------------------------------------------------------------------ mixture of experts, few tokens

@@ -212,7 +212,7 @@ void paged_decode_attention_tq_part(torch::Tensor q_rot, torch::Tensor q_jl, tor
 std::vector<torch::Tensor> token_logprobs(torch::Tensor logits, torch::Tensor tokens, int64_t top);
 std::vector<torch::Tensor> linear_logprobs(torch::Tensor x, torch::Tensor w, int64_t packed_v, torch::Tensor tokens,
                                            double softcap);
-int64_t linear_logprobs_error(bool reset);
+int64_t linear_logprobs_error(int64_t set);
 void moe_layer(torch::Tensor x, torch::Tensor router, torch::Tensor gate_up, int64_t n_gate_up, torch::Tensor down,
                int64_t n_down, int64_t k, bool renormalize, int64_t first_expert, torch::Tensor out);
 int64_t moe_layer_error(bool reset);

@@ -47,7 +47,9 @@ constexpr size_t kLlSmem = 1024 + kLlRing + kLlA + 512;
 constexpr float kLlFloor = -1e30f;       // lower bound of x - m in products with e^(x - m) = 0, which stay 0
 constexpr int64_t kLlRows = 8192;        // rows per pass: bounds the partial results (16 bytes per row and slice)
 
-static __device__ int g_ll_err;          // first error code of the bounded waits, one word per device
+// First error code of the bounded waits, one word per device. A kernel whose wait ran out leaves partial results
+// unwritten, so the rows come back as NaN until the word has been read and reset (linear_logprobs_error).
+static __device__ int g_ll_err;
 
 // Work units: row tiles x vocabulary tiles of tile_n columns, the row tiles of one vocabulary tile in a row.
 struct LlArgs {
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(kLlRowThreads) linear_logprob_rows_kernel(cons
     __syncthreads();
   }
   if (g != 0 || row >= a.T) return;
-  const bool ok = stat_valid(acc);
+  const bool ok = stat_valid(acc) && __ldcg(&g_ll_err) == 0;
   const int tok = token_id(a.tokens, row, a.V);
   float xt = NAN;
   if (tok >= 0) {
@@ -518,11 +520,12 @@ std::vector<torch::Tensor> linear_logprobs(torch::Tensor x, torch::Tensor w, int
   return {logprob, entropy};
 }
 
-int64_t linear_logprobs_error(bool reset) {
+// The device's error word; `set` >= 0 is stored in it afterwards.
+int64_t linear_logprobs_error(int64_t set) {
   int v = 0;
   B200_REQUIRE_CUDA(cudaMemcpyFromSymbol(&v, g_ll_err, sizeof(int)));
-  if (reset) {
-    const int z = 0;
+  if (set >= 0) {
+    const int z = (int)set;
     B200_REQUIRE_CUDA(cudaMemcpyToSymbol(g_ll_err, &z, sizeof(int)));
   }
   return v;

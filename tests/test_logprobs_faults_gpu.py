@@ -55,3 +55,16 @@ def test_logits_far_below_zero(packed, T):
         assert bool((lp == -(2.0 ** 100)).all() and (ent == 0).all())
         tokens[:] = 9
         assert bool((ops.linear_logprobs(x, head, tokens)[0] == 0).all())
+
+
+def test_results_are_void_until_the_error_word_is_read():
+    """After a bounded wait has run out (here: its code is put into the error word) no plausible numbers come back."""
+    x, w = torch.randn(5, 64, device=dev).bfloat16(), torch.randn(500, 64, device=dev).bfloat16()
+    tokens = torch.arange(5, device=dev)
+    good = ops.linear_logprobs(x, w, tokens)
+    assert ops.ext().linear_logprobs_error(13) == 0
+    void = ops.linear_logprobs(x, w, tokens)
+    assert all(bool(t.isnan().all()) for t in void)
+    assert ops.linear_logprobs_error(reset=False) == 13 and ops.linear_logprobs_error() == 13
+    assert ops.linear_logprobs_error() == 0
+    assert all(torch.equal(a, b) for a, b in zip(good, ops.linear_logprobs(x, w, tokens)))

@@ -102,3 +102,13 @@ def test_streaming_ignores_logprobs(engine, monkeypatch):
     for value in (5, 50, True, False, "many"):
         assert engine.generate_streaming(msgs, 4, 0.0, sampling={"top_k": 1, "logprobs": value}) == want
     assert len(seen) == 6 and all(r.params.logprobs == -1 and r.logprobs == [] for r in seen)
+
+
+def test_a_wait_that_ran_out_fails_the_score(engine, monkeypatch):
+    from b200serve import ops
+    codes = [13]
+    monkeypatch.setattr(ops, "linear_logprobs_error", lambda reset=True: codes.pop() if codes else 0)
+    with pytest.raises(RuntimeError, match="code 13"):
+        engine.score([[1, 2, 3]], timeout=60)
+    [ok] = engine.score([[1, 2, 3]], timeout=60)
+    assert len(ok["logprobs"]) == 2
