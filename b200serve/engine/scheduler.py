@@ -290,7 +290,7 @@ class Scheduler:
         req.finish_reason = reason
         req.finish_time = time.perf_counter()
         if req.blocks:
-            if req.mm is None:
+            if req.mm is None and reason != "error":    # what a failed step left in its pages is not shared
                 self.alloc.register(req.blocks, req.tokens[: req.num_computed])
             self.alloc.release(req.blocks)
             req.blocks = []

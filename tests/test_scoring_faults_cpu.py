@@ -112,3 +112,20 @@ def test_a_wait_that_ran_out_fails_the_score(engine, monkeypatch):
         engine.score([[1, 2, 3]], timeout=60)
     [ok] = engine.score([[1, 2, 3]], timeout=60)
     assert len(ok["logprobs"]) == 2
+
+
+def test_pages_of_a_failed_step_stay_out_of_the_prefix_cache(engine, monkeypatch):
+    """A step that ends in an exception after its forward may have written anything into its pages."""
+    prompt, params = list(range(200, 260)), SamplingParams(max_tokens=4, ignore_eos=True)
+
+    def failing(logits, reqs):
+        raise RuntimeError("the step's results are void")
+
+    monkeypatch.setattr(engine.scheduler, "_sample", failing)
+    [req] = engine.generate([prompt], params, timeout=60)
+    assert req.finish_reason == "error"
+    monkeypatch.undo()
+    [again] = engine.generate([prompt], params, timeout=60)
+    assert again.finish_reason == "length" and again.prefix_hit == 0
+    [third] = engine.generate([prompt], params, timeout=60)
+    assert third.prefix_hit > 0 and third.output == again.output
