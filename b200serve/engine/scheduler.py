@@ -201,6 +201,7 @@ class Scheduler:
                         if n > 1:
                             nxt = torch.as_tensor(r.tokens[1:], dtype=torch.long).to(hid.device)
                             scores = tuple(t.tolist() for t in self.runner.score(hid[off:off + n - 1], nxt))
+                            self._check_layers()
                             code = ops.linear_logprobs_error()
                             if code:
                                 raise RuntimeError(f"a wait inside the scoring kernel ran out (code {code})")
@@ -208,7 +209,9 @@ class Scheduler:
                     except Exception as e:           # (no room, say) concerns this request alone
                         r.error = e
                 else:
-                    r.embedding = hid[off:off + n].float().mean(0).cpu().tolist()
+                    pooled = hid[off:off + n].float().mean(0).cpu().tolist()
+                    self._check_layers()
+                    r.embedding = pooled
                 off += n
                 r.state, r.finish_reason = "finished", "error" if r.error is not None else "stop"
                 r.finish_time = time.perf_counter()
@@ -382,6 +385,7 @@ class Scheduler:
     def _accept_pipelined(self, batch, ev, slot) -> int:
         ev.synchronize()
         toks = self.runner.h_toks[slot][:len(batch)].tolist()
+        self._check_layers()
         n = 0
         for q, t in zip(batch, toks):
             if q.state == "finished":
@@ -438,6 +442,7 @@ class Scheduler:
         if toks is None:
             toks = self._sample_scored(logits, batch)
         toks = toks.tolist()
+        self._check_layers()
         for i, cap in watch:
             cap.finish_token(logits[i], toks[i])
         self.stats["decode_steps"] += 1
@@ -489,6 +494,7 @@ class Scheduler:
         for r, n in reqs:
             r.num_computed += n
         toks = self._sample_scored(logits, sample_reqs).tolist() if sample_reqs else []
+        self._check_layers()
         for j, (r, t) in enumerate(zip(sample_reqs, toks)):
             if r.telemetry is not None:
                 r.telemetry.finish_token(logits[j], t)
@@ -613,6 +619,7 @@ class Scheduler:
         if plain_reqs:
             toks = self._sample_scored(logits[plain_rows], plain_reqs).tolist()
             spec += [(r, [t]) for r, t in zip(plain_reqs, toks)]
+        self._check_layers()
         took = {}
         for r, new in spec:
             took[id(r)] = 0
@@ -628,6 +635,14 @@ class Scheduler:
         # MTP: rows 0..(tokens taken - 1) of each verify segment are now committed positions
         self._mtp_commit([(si, 0, r, start, took.get(id(r), 0)) for si, r, start in commits])
         return accepted
+
+    @staticmethod
+    def _check_layers():
+        """Fails the step, once its tokens are on the host and before they are taken, if a fused MoE layer gave up
+        its wait: its outputs are void. Costs a read of host memory."""
+        code = ops.moe_layer_error(wait=False)
+        if code:
+            raise RuntimeError(f"a wait inside a fused MoE layer ran out (code {code}); the step's results are void")
 
     def _sample_scored(self, logits, reqs) -> torch.Tensor:
         """``_sample``, and for requests with ``params.logprobs`` >= 0 a record of the token's log probability, rank,

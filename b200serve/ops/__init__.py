@@ -1477,9 +1477,15 @@ def moe_layer(x, router, gate_up, n_gate_up, down, n_down, k, renormalize=True, 
     return res
 
 
-def moe_layer_error(reset: bool = True) -> int:
-    """First error code of moe_layer's bounded waits on the current device (0 = none)."""
-    return int(ext().moe_layer_error(reset)) if extension_loaded() else 0
+def moe_layer_error(reset: bool = True, wait: bool = True) -> int:
+    """Error code of moe_layer's bounded wait on the current device (0 = none), over the calls on the current
+    stream; ``wait=False``: over those that have finished, without waiting for the GPU. Outputs whose wait ran out (after
+    the process-wide limit of device waits, 2 s by default) are NaN."""
+    if not extension_loaded():
+        return 0
+    if wait and torch.cuda.is_initialized():
+        torch.cuda.current_stream().synchronize()
+    return int(ext().moe_layer_error(reset))
 
 
 def gemm_error_flag(reset: bool = True) -> int:

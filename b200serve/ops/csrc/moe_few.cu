@@ -32,6 +32,9 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <algorithm>
+#include <atomic>
+#include <cstring>
+#include <mutex>
 #include "tma_host.h"
 
 namespace b200 {
@@ -41,7 +44,27 @@ constexpr int kMfWarps = 8;
 constexpr int kMfThreads = kMfWarps * 32;
 constexpr int kMfRouterThreads = 256;
 
-static __device__ int g_mf_err;                  // first error code of the bounded waits, one word per device
+constexpr int kMfWaitCode = 24;                  // error code: the wait for the gate/up units ran out
+constexpr int kMfMaxDevices = 64;
+
+// One host-mapped error word per device: a kernel whose wait runs out stores its code there, and the host reads it
+// without waiting for the GPU.
+static std::atomic<int*> g_mf_words{nullptr};
+static int* mf_error_words() {
+  static std::once_flag once;
+  std::call_once(once, [] {
+    // allowed while a graph is captured: the allocation is not part of it
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    B200_REQUIRE_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    void* p = nullptr;
+    const cudaError_t e = cudaHostAlloc(&p, kMfMaxDevices * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+    B200_REQUIRE_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    B200_REQUIRE_CUDA(e);
+    memset(p, 0, kMfMaxDevices * sizeof(int));
+    g_mf_words = static_cast<int*>(p);           // the same address on the host and on every device
+  });
+  return g_mf_words;
+}
 
 struct MfArgs {
   const __nv_bfloat16* x;                        // [T, H], row stride ldx
@@ -56,6 +79,8 @@ struct MfArgs {
   __nv_bfloat16* act;                            // [2][T * k][I] high parts, remainders
   __nv_bfloat16* out;                            // [T, H], row stride ldo
   long long ldo;
+  int* err;                                      // this device's error word
+  uint64_t wait_ns;                              // limit of the wait for the gate/up units
 };
 
 // ---------------------------------------------------------------- router logits
@@ -124,6 +149,7 @@ struct MfShared {
   uint4 ring[kDepth][8][kMfThreads];             // [chunk][block, half, rows g or g + 8][thread]
   float red[2][kMfWarps][NG * 128];              // partial sums: two units' worth
   int unit[4];                                   // the CTA's units, a ring
+  int gave_up;                                   // the wait for the gate/up units ran out
   int warp_slots[kMfWarps], warp_pairs[kMfWarps];  // active experts and pairs among each 32 local experts
   float pair_w[kMfMaxT * kMfMaxK];               // routing weight of an (expert, token) pair
   unsigned char pair_t[kMfMaxT * kMfMaxK];       // its token
@@ -197,6 +223,7 @@ __global__ void __launch_bounds__(kMfThreads, 2)
   __syncthreads();
   pdl_wait();
   if (tid == 0) {
+    sh.gave_up = 0;
     sh.unit[0] = atomicAdd(a.counters, 1);
     sh.unit[1] = atomicAdd(a.counters, 1);
   }
@@ -313,7 +340,7 @@ __global__ void __launch_bounds__(kMfThreads, 2)
   enter();
   fill(1);
 
-  bool ready = false;
+  bool ready = false, dead = false;                        // dead: the outputs of this CTA are NaN
   int done_units = 0;                                      // gate/up units of this CTA
   for (int n = 0;; ++n) {
     const int u = sh.unit[n & 3];
@@ -325,19 +352,22 @@ __global__ void __launch_bounds__(kMfThreads, 2)
         __threadfence();
         if (done_units) atomicAdd(a.counters + 1, done_units);
         if (u < total && n_active > 0) {
-          const uint64_t deadline = globaltimer_ns() + 2000000000ull;
+          const uint64_t deadline = globaltimer_ns() + a.wait_ns;
           for (uint32_t it = 1;; ++it) {
             int done;
             asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(done) : "l"(a.counters + 1) : "memory");
             if (done >= n_up) break;
             if ((it & 63u) == 0 && globaltimer_ns() > deadline) {
-              atomicExch(&g_mf_err, 24);                   // reported by moe_layer_error(); the results are void
+              sh.gave_up = 1;
+              *static_cast<volatile int*>(a.err) = kMfWaitCode;   // read by moe_layer_error()
+              __threadfence_system();
               break;
             }
           }
         }
       }
       __syncthreads();
+      dead = sh.gave_up != 0;
       ready = true;
     }
     if (u >= total) break;
@@ -461,7 +491,7 @@ __global__ void __launch_bounds__(kMfThreads, 2)
         const int idx = (t >> 3) * 128 + r * 8 + (t & 7);
         float v = sum_of(idx);
         if (PAIR) v += sum_of(idx + 4);
-        a.out[t * a.ldo + h] = __float2bfloat16_rn(v);
+        a.out[t * a.ldo + h] = __float2bfloat16_rn(dead ? NAN : v);
       }
     }
   }
@@ -524,6 +554,10 @@ void moe_layer(torch::Tensor x, torch::Tensor router, torch::Tensor gate_up, int
   a.act = reinterpret_cast<__nv_bfloat16*>(base + head);
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
   a.ldo = T > 1 ? out.stride(0) : H;
+  const int device = x.get_device();
+  TORCH_CHECK(device < kMfMaxDevices, "moe_layer: devices 0 to 63");
+  a.err = mf_error_words() + device;
+  a.wait_ns = flag_wait_ns();
   auto stream = at::cuda::getCurrentCUDAStream();
   const __nv_bfloat16* rp = reinterpret_cast<const __nv_bfloat16*>(router.data_ptr());
   const dim3 rg((unsigned)E, (unsigned)((T + 3) / 4)), rb(kMfRouterThreads);
@@ -540,11 +574,10 @@ void moe_layer(torch::Tensor x, torch::Tensor router, torch::Tensor gate_up, int
 }
 
 int64_t moe_layer_error(bool reset) {
-  int v = 0;
-  B200_REQUIRE_CUDA(cudaMemcpyFromSymbol(&v, g_mf_err, sizeof(int)));
-  if (reset) {
-    const int z = 0;
-    B200_REQUIRE_CUDA(cudaMemcpyToSymbol(g_mf_err, &z, sizeof(int)));
-  }
+  int* words = g_mf_words;
+  if (words == nullptr) return 0;                // no call so far
+  volatile int* word = words + c10::cuda::current_device();
+  const int v = *word;
+  if (reset && v) *word = 0;
   return v;
 }

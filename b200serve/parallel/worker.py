@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 
+from b200serve import ops
 from b200serve.engine.runner import PACK, unpack_static
 
 OP_DECODE, OP_PREFILL, OP_STOP, OP_LOOP, OP_PIPE_START, OP_PIPE_STEP = 1, 2, 3, 4, 5, 6
@@ -181,3 +182,6 @@ def worker_loop(runner, comm):
                 comm.gather_vocab(logits)
         else:
             raise RuntimeError(f"unknown step op {op}")
+        code = ops.moe_layer_error(wait=False)       # of the steps that have finished
+        if code:
+            raise RuntimeError(f"a wait inside a fused MoE layer ran out (code {code})")

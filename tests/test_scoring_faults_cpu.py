@@ -129,3 +129,41 @@ def test_pages_of_a_failed_step_stay_out_of_the_prefix_cache(engine, monkeypatch
     assert again.finish_reason == "length" and again.prefix_hit == 0
     [third] = engine.generate([prompt], params, timeout=60)
     assert third.prefix_hit > 0 and third.output == again.output
+
+
+def test_a_layer_that_gave_up_fails_its_step(engine, monkeypatch):
+    """The error word of the fused MoE layer is looked at before a step's tokens, embeddings or scores are taken."""
+    from b200serve import ops
+    codes, asked = [], []
+
+    def error(reset=True, wait=True):
+        asked.append(wait)
+        return codes.pop() if codes else 0
+
+    monkeypatch.setattr(ops, "moe_layer_error", error)
+    prompt = list(range(300, 330))
+    for params in (SamplingParams(max_tokens=4, ignore_eos=True), SamplingParams(max_tokens=4, logprobs=2)):
+        codes.append(24)
+        [req] = engine.generate([prompt], params, timeout=60)
+        assert req.finish_reason == "error" and req.output == []
+        [req] = engine.generate([prompt], params, timeout=60)
+        assert req.finish_reason in ("length", "stop") and req.prefix_hit in (0, 16)
+    codes.append(24)
+    with pytest.raises(RuntimeError, match="code 24"):
+        engine.score([[1, 2, 3]], timeout=60)
+    codes.append(24)
+    with pytest.raises(RuntimeError, match="embedding failed"):
+        engine.embed(["a few words"], timeout=60)
+    assert asked and not any(asked)                          # never waits for the GPU
+
+
+def test_a_worker_rank_stops_after_a_layer_gave_up(monkeypatch):
+    from types import SimpleNamespace
+
+    from b200serve import ops
+    from b200serve.parallel import worker
+    monkeypatch.setattr(ops, "moe_layer_error", lambda reset=True, wait=True: 24)
+    comm = SimpleNamespace(broadcast=lambda t, src: t.copy_(torch.tensor([worker.OP_PIPE_STEP] + [0] * (len(t) - 1))))
+    runner = SimpleNamespace(device="cpu", pipeline_step=lambda slot: None)
+    with pytest.raises(RuntimeError, match="code 24"):
+        worker.worker_loop(runner, comm)
