@@ -440,11 +440,20 @@ __global__ void __launch_bounds__(kMfThreads, 2)
               b[j][i] = in && k0 + 32 * i < a.I ? *reinterpret_cast<const uint4*>(arow + j * act_rows * a.I + 32 * i)
                                                 : zero;
           if (!have_w) take_w();
+          float part[2][4];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) part[i >> 2][i & 3] = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < PARTS; ++j)
-              mma_piece(acc[q][PARTS == 1 ? i & 1 : j], w[i >> 1][i & 1][0], w[i >> 1][i & 1][1], b[j][i]);
+              mma_piece(part[PARTS == 1 ? i & 1 : j], w[i >> 1][i & 1][0], w[i >> 1][i & 1][1], b[j][i]);
+          // only the expert's own tokens take its products: 0 times an infinite weight is not 0
+          const int c0 = q * 8 + (PAIR ? 2 * t4 & 3 : 2 * t4);
+          const bool in0 = m >> c0 & 1u, in1 = m >> (c0 + 1) & 1u;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i & 1 ? in1 : in0) acc[q][i >> 2][i & 3] += part[i >> 2][i & 3];
         }
       }
       out_slot = out_slot + 1 == DEPTH ? 0 : out_slot + 1;
