@@ -489,10 +489,12 @@ __global__ void __launch_bounds__(kMfThreads, 2)
         const int idx = (p >> 3) * 128 + c * 8 + (p & 7), pair = sh.slot_off[us] + p;
         const float gate = sum_of(idx), upv = sum_of(idx + 64);
         const float v = gate / (1.f + __expf(-gate)) * upv * sh.pair_w[pair];
-        const __nv_bfloat16 h = __float2bfloat16_rn(v);
+        // a finite value may round up to infinity: cut instead, the remainder has the rest. Infinity has no remainder.
+        __nv_bfloat16 h = __float2bfloat16_rn(v);
+        if (__hisinf(h)) h = __float2bfloat16_rz(v);
         __nv_bfloat16* dst = a.act + (size_t)pair * a.I + (u - us * col_blocks) * 8 + c;
         dst[0] = h;
-        dst[act_rows * a.I] = __float2bfloat16_rn(v - __bfloat162float(h));
+        dst[act_rows * a.I] = __float2bfloat16_rn(__hisinf(h) ? 0.f : v - __bfloat162float(h));
       }
     } else {
       const int r = tid & 15, t = tid >> 4, h = (u - n_up) * 16 + r;   // output row, token

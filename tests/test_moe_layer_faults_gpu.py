@@ -58,3 +58,26 @@ def test_an_experts_bad_weight_reaches_only_its_own_tokens(T, value):
         bad[2][e * (a[2].shape[0] // c.E) + 3, 5] = value    # gate row 3 of the expert
         got = ops.moe_layer(*bad)
         assert torch.equal(got[~own], good[~own]) and not bool(got[own].isfinite().all(-1).any())
+
+
+@pytest.mark.parametrize("T", [1, 6, 16])
+@pytest.mark.parametrize("up", [1.4140625 * 2.0 ** 64, -1.4140625 * 2.0 ** 64, 2.0 ** 90, -2.0 ** 90])
+def test_activations_at_the_end_of_the_range(T, up):
+    """silu(1.4140625 * 2^63) * up: +-1.99957 * 2^127 lies between bf16's largest value and fp32's (the output is
+    exact to bf16's rounding), with 2^90 it is +-infinity (the output has the down weight's sign)."""
+    c = MoECase(T=T, H=64, E=1, k=1, inner=1)
+    g = torch.Generator().manual_seed(1)
+    c.x.zero_()
+    c.x[:, 0] = 1.0
+    size = torch.randint(64, 128, (c.H,), generator=g) * 2.0 ** -17          # 8-bit factors of 2^-11 to 2^-10
+    down = (size * torch.where(torch.rand(c.H, generator=g) < 0.5, -1.0, 1.0)).bfloat16()
+    a = list(c.args(dev))
+    tiles_gu, tiles_dn = torch.zeros_like(a[2]), torch.zeros_like(a[4])
+    tiles_gu[0, 0], tiles_gu[64, 0] = 1.4140625 * 2.0 ** 63, up              # gate row 0, up row 0
+    tiles_dn[:c.H, 0] = down.to(dev)
+    a[2], a[4] = tiles_gu, tiles_dn
+    act = torch.tensor(1.4140625 * 2.0 ** 63, dtype=torch.float64) * up
+    if abs(up) == 2.0 ** 90:
+        act = act.sign() * INF
+    want = (act * down.double()).bfloat16().expand(T, -1)
+    assert torch.equal(ops.moe_layer(*a).cpu(), want)
