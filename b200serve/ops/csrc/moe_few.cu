@@ -90,16 +90,14 @@ __global__ void __launch_bounds__(kMfRouterThreads) moe_router_kernel(const __nv
   __shared__ float red[kMfRouterThreads / 32][TT];
   const int e = blockIdx.x, tid = threadIdx.x, t0 = blockIdx.y * TT;
   const __nv_bfloat16* w = router + (size_t)e * a.H;
-  bf16x8 first{};                                // a weight: does not depend on the previous kernel
-  if (tid * 8 < a.H) first = *reinterpret_cast<const bf16x8*>(w + tid * 8);
   pdl_trigger();
-  pdl_wait();
+  pdl_wait();                                    // the previous kernel may have written the router itself
   if (e == 0 && t0 == 0 && tid < 2) counters[tid] = 0;
   float acc[TT];
 #pragma unroll
   for (int t = 0; t < TT; ++t) acc[t] = 0.f;
   for (int i = tid * 8; i < a.H; i += kMfRouterThreads * 8) {
-    const bf16x8 wv = i == tid * 8 ? first : *reinterpret_cast<const bf16x8*>(w + i);
+    const bf16x8 wv = *reinterpret_cast<const bf16x8*>(w + i);
     bf16x8 xv[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t)                 // rows past T repeat the last one: loads without branches

@@ -81,3 +81,37 @@ def test_activations_at_the_end_of_the_range(T, up):
         act = act.sign() * INF
     want = (act * down.double()).bfloat16().expand(T, -1)
     assert torch.equal(ops.moe_layer(*a).cpu(), want)
+
+
+@pytest.mark.parametrize("T", [1, 16])
+def test_a_router_written_by_the_kernel_before(T):
+    """The router is an operand like the rows: a kernel right before the call, which lets the next one start early,
+    may write it."""
+    c = MoECase(T=T, H=2048, E=32, k=4, inner=64)
+    a = list(c.args(dev))
+    g = torch.Generator(device=dev).manual_seed(3)
+    sources = [torch.randn(32, 2048, device=dev, generator=g).bfloat16() for _ in range(6)]
+    scale = torch.full((2048,), 0.03, device=dev, dtype=torch.bfloat16)
+    want = []
+    for s in sources:
+        a[1] = ops.rmsnorm(s, scale, 1e-6).clone()
+        torch.cuda.synchronize()
+        want.append(ops.moe_layer(*a))
+    a[1] = torch.zeros(32, 2048, device=dev, dtype=torch.bfloat16)
+
+    def passes():
+        out = []
+        for s in sources:
+            ops.rmsnorm(s, scale, 1e-6, out=a[1])
+            out.append(ops.moe_layer(*a))
+        return out
+
+    eager = passes()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = passes()
+    for _ in range(5):
+        graph.replay()
+    torch.cuda.synchronize()
+    for outs in (eager, captured):
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
