@@ -1435,7 +1435,8 @@ def moe_layer(x, router, gate_up, n_gate_up, down, n_down, k, renormalize=True, 
     experts first_expert, first_expert + 1, ... packed by models.moe.pack_experts (gate and up
     interleaved by 64 rows, ``n_gate_up`` rows per expert; ``n_down`` = H rows), or the
     tensors it returns. ``renormalize``: the k weights sum to 1. Experts of other ranks add
-    nothing; a row that has none here comes back as zeros. Returns [T, H]."""
+    nothing; a row that has none here comes back as zeros. Returns [T, H] (``out``: rows may be strided but not
+    overlap; it may be x itself)."""
     T, H = x.shape
     if T > MOE_LAYER_MAX_ROWS:
         raise ValueError(f"moe_layer: at most {MOE_LAYER_MAX_ROWS} rows, got {T}")

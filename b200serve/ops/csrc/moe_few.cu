@@ -543,8 +543,8 @@ void moe_layer(torch::Tensor x, torch::Tensor router, torch::Tensor gate_up, int
                "moe_layer: experts [" + std::to_string(first_expert) + ", " + std::to_string(first_expert + local) +
                    ") are not among the router's " + std::to_string(E));
   TORCH_CHECK(out.dim() == 2 && out.size(0) == T && out.size(1) == H && out.scalar_type() == at::kBFloat16 &&
-                  out.stride(1) == 1 && out.device() == x.device(),
-              "moe_layer: out must be a bf16 tensor [T, H] on x's device");
+                  out.stride(1) == 1 && (T <= 1 || out.stride(0) >= H) && out.device() == x.device(),
+              "moe_layer: out must be a bf16 tensor [T, H] on x's device whose rows do not overlap");
   if (T == 0) return;
   const c10::cuda::CUDAGuard guard(x.device());
   // this call's scratch: router logits, two counters, the activations of T * k pairs

@@ -115,3 +115,15 @@ def test_a_router_written_by_the_kernel_before(T):
     torch.cuda.synchronize()
     for outs in (eager, captured):
         assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_out_may_be_x_and_its_rows_may_not_overlap():
+    c = MoECase(T=9, H=256, E=12, k=3, inner=96)
+    a = list(c.args(dev))
+    want = ops.moe_layer(*a)
+    for bad in (torch.empty(1, 256, device=dev).bfloat16().expand(9, -1),
+                torch.empty(4096, device=dev).bfloat16().as_strided((9, 256), (128, 1))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.moe_layer(*a, out=bad)
+    same = a[0] = a[0].clone()
+    assert ops.moe_layer(*a, out=same) is same and torch.equal(same, want)
