@@ -1395,7 +1395,7 @@ def token_logprobs(logits, tokens, top=0) -> TokenLogprobs:
 def linear_logprobs(x, w, tokens, softcap=0.0):
     """(log probability of ``tokens`` [T], entropy [T]) fp32 of the rows of x @ w^T without storing
     the logits: x [T, H] bf16 (H a multiple of 8, rows may be strided), w the LM head [V, H] bf16, plain or
-    a PackedWeight, tokens int32 / int64. ``softcap`` > 0: logits become
+    a PackedWeight, tokens int32 / int64. ``softcap`` > 0 (2^-100 to 2^100): logits become
     softcap * tanh(logit / softcap). An id outside [0, V) has log probability NaN (its entropy is
     computed); a row whose logits hold a NaN or +inf has NaN for both. A quantised LM head takes
     linear() and token_logprobs()."""
@@ -1406,8 +1406,8 @@ def linear_logprobs(x, w, tokens, softcap=0.0):
         raise TypeError(f"linear_logprobs: w must be a tensor or a PackedWeight, got {type(w).__name__}")
     if x.shape[1] != w.shape[1]:
         raise ValueError(f"linear_logprobs: x has {x.shape[1]} columns, w {w.shape[1]}")
-    if not 0 <= softcap < math.inf:
-        raise ValueError(f"linear_logprobs: softcap must be finite and not negative, got {softcap}")
+    if not (softcap == 0 or 2.0 ** -100 <= softcap <= 2.0 ** 100):     # its reciprocal is held in fp32
+        raise ValueError(f"linear_logprobs: softcap must be 0 (off) or 2^-100 to 2^100, got {softcap}")
     if _cuda(x, 2):
         return tuple(ext().linear_logprobs(x, w.data if packed else w, w.N if packed else 0, tokens, float(softcap)))
     logits = x.float() @ (w.unpacked() if packed else w).float().t()

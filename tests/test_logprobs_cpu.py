@@ -94,3 +94,12 @@ def test_refusals():
                 but(_4=a[4][:-1]), but(_8=1), but(_8=-1)):
         with pytest.raises(ValueError):
             ops.moe_layer(*bad)
+
+
+def test_softcap_whose_reciprocal_fp32_cannot_hold():
+    h, w, tok = torch.zeros(2, 16).bfloat16(), torch.zeros(10, 16).bfloat16(), torch.zeros(2, dtype=torch.int64)
+    for cap in (1e-300, 1e-45, 1e-39, 1e39, 1e300):
+        with pytest.raises(ValueError, match="softcap"):
+            ops.linear_logprobs(h, w, tok, softcap=cap)
+    for cap in (0, 2.0 ** -100, 2.0 ** 100):
+        assert all(bool(t.isfinite().all()) for t in ops.linear_logprobs(h, w, tok, softcap=cap))

@@ -68,3 +68,14 @@ def test_results_are_void_until_the_error_word_is_read():
     assert ops.linear_logprobs_error(reset=False) == 13 and ops.linear_logprobs_error() == 13
     assert ops.linear_logprobs_error() == 0
     assert all(torch.equal(a, b) for a, b in zip(good, ops.linear_logprobs(x, w, tokens)))
+
+
+def test_softcap_at_the_ends_of_its_range():
+    x, w = torch.randn(9, 64, device=dev).bfloat16(), torch.randn(500, 64, device=dev).bfloat16()
+    tokens = torch.arange(9, device=dev)
+    got, plain = ops.linear_logprobs(x, w, tokens, softcap=2.0 ** 100), ops.linear_logprobs(x, w, tokens)
+    assert all(torch.equal(a, b) for a, b in zip(got, plain))            # powers of two: the same bits
+    lp, ent = ops.linear_logprobs(x, w, tokens, softcap=2.0 ** -100)     # every logit next to 0: uniform
+    want = math.log(500)
+    assert float((lp + want).abs().max()) < log_s_bound(500) + want * 2.0 ** -22
+    assert float((ent - want).abs().max()) < entropy_bound(500)
