@@ -449,6 +449,8 @@ std::vector<torch::Tensor> linear_logprobs(torch::Tensor x, torch::Tensor w, int
   const c10::cuda::CUDAGuard guard(x.device());
   auto logprob = torch::empty({T}, x.options().dtype(at::kFloat)), entropy = torch::empty_like(logprob);
   if (T == 0) return {logprob, entropy};
+  // rows that lie on one another (an expanded or windowed tensor) are copied out: TMA takes rows side by side
+  if (T > 1 && x.stride(0) < H) x = x.contiguous();
   const int64_t ldx = T > 1 ? x.stride(0) : H;
   TORCH_CHECK(ldx % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0,
               "linear_logprobs: rows of x must start on 16-byte boundaries");

@@ -79,3 +79,14 @@ def test_softcap_at_the_ends_of_its_range():
     want = math.log(500)
     assert float((lp + want).abs().max()) < log_s_bound(500) + want * 2.0 ** -22
     assert float((ent - want).abs().max()) < entropy_bound(500)
+
+
+def test_rows_that_overlap_in_memory():
+    """x.expand() and windows of one buffer: legal strides, and every row is what indexing says."""
+    w = torch.randn(700, 128, device=dev).bfloat16()
+    buf = torch.randn(4096, device=dev).bfloat16()
+    for T in (5, 150):
+        tokens = torch.randint(0, 700, (T,), device=dev)
+        for x in (buf[:128].expand(T, -1), buf.as_strided((T, 128), (8, 1)), buf.as_strided((T, 128), (4, 1))):
+            got, want = ops.linear_logprobs(x, w, tokens), ops.linear_logprobs(x.clone().contiguous(), w, tokens)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
