@@ -1,0 +1,82 @@
+"""LM-head scoring at the sizes and with the options that users run: the error that its split sums are for, tiles of
+two CTAs with capped logits, hidden sizes that leave a part and a block unfilled, a whole vocabulary."""
+
+import math
+
+import pytest
+import torch
+
+from b200serve import ops
+from logprob_cases import check_linear_logprobs
+
+pytestmark = pytest.mark.gpu
+dev = "cuda"
+
+
+@pytest.fixture(autouse=True)
+def _seed():
+    torch.manual_seed(0)
+    ops.ext()
+
+
+def _stats64(x, w, tokens):
+    """In 64 bits, on the GPU: log probability, entropy, the logits' root mean square and largest spread in a row."""
+    logits = torch.cat([x.double() @ p.double().t() for p in w.split(16384)], 1)
+    logp = torch.log_softmax(logits, -1)
+    return (logp.gather(1, tokens[:, None])[:, 0], -(logp.exp() * logp).sum(-1), logits.pow(2).mean().sqrt().item(),
+            logits.std(-1).max().item())
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("T", [100, 300])
+def test_error_of_the_split_sums(packed, T):
+    """Root-mean-square error of the log probabilities at H = 4096 beside that of the logits.
+
+    The tensor cores cut each addition of 16 products, by half a last place of the running sum on average and always
+    towards zero: after n of them a sum of size r is off by about n 2^-24 (2/3) r. In parts of 512 elements
+    n = 32 and r = sqrt(512 / 4096) of the logit; eight parts of either sign make 32 * 2^-24 * 2/3 * 0.354 * sqrt(8) =
+    1.3e-6 of the logit (0.9e-6 for 256). A log probability takes two such logits, the token's and, where one dominates, the
+    largest: sqrt 2 of it, 1.8e-6. One sum over H would have n = 256: 1.0e-5 for a logit, 1.4e-5."""
+    H, V = 4096, 320
+    x = torch.randn(T, H, device=dev).bfloat16()
+    w = (torch.randn(V, H, device=dev) * 8.0 / math.sqrt(H)).bfloat16()       # logits of root mean square 8
+    tokens = torch.randint(0, V, (T,), device=dev)
+    want, _, rms, _ = _stats64(x, w, tokens)
+    lp, _ = ops.linear_logprobs(x, ops.PackedWeight(w) if packed else w, tokens)
+    err = (lp.double() - want).pow(2).mean().sqrt().item()
+    assert 6 < rms < 10 and err < 2e-6 * rms, (err / rms)
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("T", [5, 129, 200, 300])
+def test_softcap_and_unfilled_parts(packed, T):
+    """H = 1608 is 26 blocks of 64, the last one of 8: parts of 4 or 8 blocks with a remainder of 2. T > 128 takes two
+    CTAs per tile."""
+    V, H = 3001, 1608
+    w = (torch.randn(V, H, device=dev) * 20.0 / math.sqrt(H)).bfloat16()
+    x = torch.randn(T, H, device=dev).bfloat16()
+    tokens = torch.randint(0, V, (T,), device=dev)
+    head = ops.PackedWeight(w) if packed else w
+    for cap in (0.0, 15.0):
+        check_linear_logprobs(ops.linear_logprobs(x, head, tokens, softcap=cap), x, w, tokens, cap)
+    assert ops.linear_logprobs_error() == 0
+
+
+@pytest.mark.parametrize("T", [1, 23, 700])
+def test_a_whole_vocabulary(T):
+    """151936 tokens of 4096 elements. Per logit the parts above leave 1.3e-6 of its size, so 5 times that for the
+    largest of T * V (their errors are sums of many terms); the entropy's derivative is bounded by 2 ln V, and the sums
+    over V add the bounds of the shared statistics."""
+    from logprob_cases import entropy_bound, logprob_bound
+    V, H = 151936, 4096
+    w = (torch.randn(V, H, device=dev) * 1.3 / math.sqrt(H)).bfloat16()
+    tokens = torch.randint(0, V, (T,), device=dev)
+    x = (torch.randn(T, H, device=dev) + torch.rand(T, 1, device=dev) * 8 * w[tokens].float()).bfloat16()
+    want, ent, _, spread = _stats64(x, w, tokens)
+    logit_err = 5 * 1.3e-6 * max(spread, 16.0)               # the token's own logit reaches 8 * 1.3^2 + 3
+    lp, en = ops.linear_logprobs(x, ops.PackedWeight(w), tokens)
+    assert float((lp.double() - want).abs().max()) < logprob_bound(V, float(want.abs().max()), logit_err)
+    assert float((en.double() - ent).abs().max()) < entropy_bound(V, logit_err)
+    two = ops.token_logprobs(ops.linear(x, ops.PackedWeight(w), epilogue=ops.EPI_F32), tokens)
+    # linear() keeps one sum over H: 1.0e-5 of a logit on average
+    assert float((lp - two.logprob).abs().max()) < 5 * 2 * 1.0e-5 * 16.0
