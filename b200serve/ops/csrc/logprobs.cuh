@@ -5,8 +5,9 @@
 // Slices join exactly: with M = max m_i and d_i = m_i - M,
 //   s = sum e^d_i s_i,   t = sum e^d_i (t_i + d_i s_i),
 //   log p(token) = (x_token - M) - log s,   entropy = log s - t / s.
-// Everything is fp32: every term lies in [0, 1], so a sum of V of them keeps a relative error of a
-// few 2^-24, and the differences from the maximum are exact to half an ulp.
+// Everything is fp32. The terms of s lie in [0, 1] and those of t in [-1/e, 0]. An exponential carries ex2's 2^-22 and
+// the rounding of its argument d log2(e), 2^-23 |d| (|d| <= ln V where it matters), so log s is off by
+// about (1 + ln V) 2^-22; the sums, of at most 64 terms in a row and joined in trees, add a few 2^-24.
 #pragma once
 #include "common.cuh"
 

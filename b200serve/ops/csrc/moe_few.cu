@@ -25,9 +25,9 @@
 //
 // Numerics: fp32 accumulation; the routing weight is folded into the activation in fp32, and the
 // activation is kept as the sum of two bf16 (high part and remainder, 16 bits of mantissa), so
-// the only rounding at bf16 precision is that of the output. Stage s of a unit always goes through
-// the same partial sum and partial sums join in the order of s, whichever CTA or warp ran it:
-// equal inputs give equal bits.
+// the only rounding at bf16 precision is that of the output. Chunk c of a unit always goes to warp c mod 8,
+// a warp adds its chunks in their order and the warps' sums join in the order of the warps, whichever CTA
+// took the unit: equal inputs give equal bits.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
