@@ -127,3 +127,38 @@ def test_out_may_be_x_and_its_rows_may_not_overlap():
             ops.moe_layer(*a, out=bad)
     same = a[0] = a[0].clone()
     assert ops.moe_layer(*a, out=same) is same and torch.equal(same, want)
+
+
+_FIRST_CALL = """
+import sys
+sys.path[:0] = ["tests", "."]
+import torch
+from b200serve import ops
+from logprob_cases import MoECase
+c = MoECase(T=5, H=256, E=8, k=2, inner=64)
+a = c.args("cuda")
+x, w, t = torch.randn(5, 64, device="cuda").bfloat16(), torch.randn(300, 64, device="cuda").bfloat16(), \\
+    torch.arange(5, device="cuda")
+ops.ext()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out, (lp, ent) = ops.moe_layer(*a), ops.linear_logprobs(x, w, t)
+    tok = ops.token_logprobs(x.float(), t, top=3)
+g.replay()
+torch.cuda.synchronize()
+ref, bound = c.reference()
+assert bool(((out.double().cpu() - ref).abs() <= bound).all()) and ops.moe_layer_error() == 0
+assert all(torch.equal(p, q) for p, q in zip((lp, ent), ops.linear_logprobs(x, w, t)))
+assert all(torch.equal(p, q) for p, q in zip(tok, ops.token_logprobs(x.float(), t, top=3)))
+print("captured")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    """What a process sets up once (the error words, the kernels' attributes) is allowed inside a capture."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
