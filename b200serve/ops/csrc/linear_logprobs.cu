@@ -19,7 +19,7 @@
 //
 // Sums over H. The tensor cores cut the bits that do not fit when they add to an fp32 accumulator, so
 // the error of one long sum grows with H and has a sign: 5.5e-6 of the result's norm at H = 4096, five
-// times a rounded fp32 sum's. So only 256 or 512 elements are summed up in TMEM; the epilogue adds these
+// times a rounded fp32 sum's. So only 128 or 512 elements are summed up in TMEM; the epilogue adds these
 // parts to the 128 sums that each of its threads keeps in registers, rounding to nearest. The two TMEM
 // buffers alternate between parts, and the MMAs run on under the epilogue.
 //
@@ -484,9 +484,12 @@ std::vector<torch::Tensor> linear_logprobs(torch::Tensor x, torch::Tensor w, int
     a.per_tile = a.tile_n > kLlCols ? 2 : 1;
     const int64_t slices = (int64_t)a.v_tiles * a.per_tile;
     a.inv_softcap = softcap > 0.0 ? (float)(1.0 / softcap) : 0.f;
-    // 256 elements per part where the read of w is the bound, else 512 (the epilogue's additions then stay under the
-    // MMAs: 2048 rows of H = 4096 take 2.10 ms instead of 2.29)
-    a.part_kb = cg == 1 ? 4 : 8;
+    // 128 elements per part where the read of w is the bound, else 512 (the epilogue's additions then stay under the
+    // MMAs: 2048 rows of H = 4096 take 2.00 ms, parts of 256 2.18). Root-mean-square error of a log probability, logits
+    // up to 15: 6.2e-7 for 128, 9.0e-7 for 256, 1.8e-6 for 512 elements (a rounded fp32 product 3.8e-6, one row of it
+    // 3.7e-7); below 128 the roundings of the many additions take over. One row of 151936 x 4096: 201 us,
+    // with parts of 256 195, of 64 228.
+    a.part_kb = cg == 1 ? 2 : 8;
     a.softcap = (float)softcap;
     const bool is64 = tokens.scalar_type() == at::kLong;
     a.tokens = TokenIds{static_cast<const char*>(tokens.data_ptr()) + t0 * (is64 ? 8 : 4), is64};

@@ -35,7 +35,7 @@ def test_error_of_the_split_sums(packed, T):
     The tensor cores cut each addition of 16 products, by half a last place of the running sum on average and always
     towards zero: after n of them a sum of size r is off by about n 2^-24 (2/3) r. In parts of 512 elements
     n = 32 and r = sqrt(512 / 4096) of the logit; eight parts of either sign make 32 * 2^-24 * 2/3 * 0.354 * sqrt(8) =
-    1.3e-6 of the logit (0.9e-6 for 256). A log probability takes two such logits, the token's and, where one dominates, the
+    1.3e-6 of the logit (less for shorter parts). A log probability takes two such logits, the token's and, where one dominates, the
     largest: sqrt 2 of it, 1.8e-6. One sum over H would have n = 256: 1.0e-5 for a logit, 1.4e-5."""
     H, V = 4096, 320
     x = torch.randn(T, H, device=dev).bfloat16()
@@ -80,3 +80,19 @@ def test_a_whole_vocabulary(T):
     two = ops.token_logprobs(ops.linear(x, ops.PackedWeight(w), epilogue=ops.EPI_F32), tokens)
     # linear() keeps one sum over H: 1.0e-5 of a logit on average
     assert float((lp - two.logprob).abs().max()) < 5 * 2 * 1.0e-5 * 16.0
+
+
+def test_few_rows_are_as_exact_as_a_rounded_product():
+    """Up to 128 rows take parts of 128 elements. As above, 8 cuts leave 8 * 2^-24 * 2/3 * sqrt(128 / 4096) = 5.6e-8 of the
+    logit, sqrt(32) times that over 32 parts of either sign: 3.2e-7; the 32 rounded additions of a growing sum leave
+    2^-24 / sqrt 3 * sqrt(32 / 3) = 1.1e-7. Together 3.4e-7, sqrt 2 of it for the two logits that count: 4.8e-7 (with a
+    last place of 2^-23 throughout, its upper end). Parts of 256 elements measure 5.4e-7, of 128 3.6e-7."""
+    H, V, T = 4096, 64, 128
+    w = (torch.randn(V, H, device=dev) * 8.0 / math.sqrt(H)).bfloat16()
+    x = torch.randn(T, H, device=dev).bfloat16()
+    tokens = torch.randint(0, V, (T,), device=dev)
+    want, _, rms, _ = _stats64(x, w, tokens)
+    err = torch.cat([ops.linear_logprobs(x[i:i + 1], w, tokens[i:i + 1])[0] for i in range(T)]).double() - want
+    assert err.pow(2).mean().sqrt().item() < 4.8e-7 * rms
+    lp, _ = ops.linear_logprobs(x, w, tokens)
+    assert (lp.double() - want).pow(2).mean().sqrt().item() < 4.8e-7 * rms
