@@ -62,7 +62,7 @@ struct LlArgs {
   float softcap, inv_softcap;
   TokenIds tokens;
   int per_tile;                          // slices of up to 128 columns in a tile: 1 or 2
-  float4* part;                          // [v_tiles * per_tile][T] (m, s, t, the token's logit where the slice has it)
+  float4* part;                          // [v_tiles * per_tile][T] (m, r, t, the token's logit where the slice has it)
 };
 
 // TMA maps of w with boxes of 16, 32, 48, ... 128 rows: a tile of a packed weight takes one box per 128-row
@@ -342,8 +342,21 @@ __global__ void __launch_bounds__(kLlThreads, 1)
         t[j & 3] = fmaf(e, fmaxf(d, kLlFloor), t[j & 3]);  // a logit of -inf: 0 * -1e30
       }
       const float ss = (s[0] + s[1]) + (s[2] + s[3]), tt = (t[0] + t[1]) + (t[2] + t[3]);
+      // the maximum's own term leaves the sum: by subtraction, or, where that would cost the others' bits, by another
+      // sum of the others
+      float rest = ss - 1.f;
+      if (ss < 2.f && in > 0) {
+        float o[2] = {0.f, -1.f};                          // the others' terms; how many are 1, but for one
+#pragma unroll
+        for (int j = 0; j < kLlCols; ++j) {
+          const float e = ex2_in_order((v[j] - mm) * L2E);
+          if (e == 1.f) o[1] += 1.f;
+          else o[0] += e;
+        }
+        rest = o[0] + o[1];
+      }
       if (row < a.T)
-        a.part[(size_t)(x.v_tile * a.per_tile + half) * a.T + row] = make_float4(ss == ss ? m[0] : INFINITY, ss, tt, xt);
+        a.part[(size_t)(x.v_tile * a.per_tile + half) * a.T + row] = make_float4(ss == ss ? m[0] : INFINITY, rest, tt, xt);
     }
   }
   tc::tc_fence_before();
@@ -391,15 +404,20 @@ __global__ void __launch_bounds__(kLlRowThreads) linear_logprob_rows_kernel(cons
         M = fmaxf(M, p[j].x);
       }
       if (M == -INFINITY) continue;                    // nothing yet
-      float d = fmaxf(acc.m - M, kLlFloor), e = __expf(d), s = e * acc.s, t = e * (acc.t + d * acc.s);
+      float d = fmaxf(acc.m - M, kLlFloor), e = __expf(d), rest = e * acc.r, t = e * (acc.t + d * (1.f + acc.r));
+      int ones = 0;                                    // slices whose maximum is M
+      if (acc.m == M) ++ones;
+      else rest += e;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         d = fmaxf(p[j].x - M, kLlFloor);               // an empty slice: e = 0
         e = __expf(d);
-        s += e * p[j].y;
-        t += e * (p[j].z + d * p[j].y);
+        rest += e * p[j].y;
+        if (p[j].x == M) ++ones;
+        else rest += e;
+        t += e * (p[j].z + d * (1.f + p[j].y));
       }
-      acc = RowStat{M, s, t};
+      acc = RowStat{M, rest + (float)(ones - 1), t};
     }
   }
   st[g][r] = acc;
@@ -420,7 +438,7 @@ __global__ void __launch_bounds__(kLlRowThreads) linear_logprob_rows_kernel(cons
     const int v_tile = tok / a.tile_n, half = (tok - v_tile * a.tile_n) / kLlCols;
     xt = __ldcg(&a.part[(size_t)(v_tile * a.per_tile + half) * a.T + row].w);
   }
-  logprob[row] = ok ? (xt - acc.m) - logf(acc.s) : NAN;
+  logprob[row] = ok ? (xt - acc.m) - stat_log(acc) : NAN;
   entropy[row] = ok ? stat_entropy(acc) : NAN;
 }
 

@@ -5,7 +5,7 @@
 //   * logprob_slices: one CTA of 256 threads per (row, slice). A thread keeps its 32 logits
 //     of the slice in registers, so the maximum, the sums, the rank count and the selection all
 //     work on one read. With rows for every SM it is bound by instruction issue (about 25 a logit):
-//     256 x 248320 fp32 with top 20 take 80 us, 3.2 TB/s.
+//     256 x 248320 fp32 with top 20 take 82 us, 3.1 TB/s.
 //   * logprob_rows: one CTA per row joins the slices' statistics and merges their sorted lists.
 //
 // Selection. With the slice's logits in 32 groups (a lane of every warp), the `top`-th largest group
@@ -48,11 +48,11 @@ struct LpArgs {
   long long ld;                          // elements between rows
   int V, S, top;                         // vocabulary, slices per row, alternatives
   TokenIds tokens;
-  float4* part;                          // [B][S] (m, s, t, count of logits above the token's)
+  float4* part;                          // [B][S] (m, r, t, count of logits above the token's)
   unsigned long long* keys;              // [B][S][top] descending, 0 = none
 };
 
-// T = float or __nv_bfloat16. 32 logits per thread in 64 registers, four CTAs per SM: 16 of them take 114 us instead of
+// T = float or __nv_bfloat16. 32 logits per thread in 64 registers, four CTAs per SM: 16 of them took 114 us instead of
 // 80 for 256 x 248320 fp32 with top 20 (twice the selections), 64 of them 127 instead of 97 in bf16 (half the CTAs).
 template <typename T>
 __global__ void __launch_bounds__(kLpThreads, 4) logprob_slices_kernel(const LpArgs a) {
@@ -159,6 +159,22 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprob_slices_kernel(const LpA
   }
   s = warp_sum(s);
   t = warp_sum(t);
+  if (__any_sync(0xffffffffu, tm == m)) {
+    // the maximum's own terms are counted in the upper half of cnt and leave the sum: by subtraction, or, where that
+    // would cost the others' bits, by another sum of the others
+    if (s < 2.f && m > -INFINITY) {
+      s = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (v[i] == m) cnt += 1 << 16;
+        else s += ex2((v[i] - m) * 1.4426950408889634f);
+      }
+      s = warp_sum(s);
+    } else {
+      s -= 1.f;
+      if (lane == 0) cnt += 1 << 16;
+    }
+  }
   cnt = __reduce_add_sync(0xffffffffu, cnt);
   if (lane == 0) { red[warp][0] = s; red[warp][1] = t; red[warp][2] = __int_as_float(cnt); }
   __syncthreads();
@@ -167,8 +183,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprob_slices_kernel(const LpA
     int bc = 0;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) { bs += red[i][0]; bt += red[i][1]; bc += __float_as_int(red[i][2]); }
-    // a NaN (of the data, or +inf - +inf) marks the row through m = +inf
-    a.part[row * a.S + slice] = make_float4(bs == bs ? m : INFINITY, bs, bt, __int_as_float(bc));
+    // a NaN marks the row through m = +inf
+    a.part[row * a.S + slice] = make_float4(bs == bs ? m : INFINITY, bs + (float)((bc >> 16) - 1), bt,
+                                            __int_as_float(bc & 0xffff));
   }
   if (a.top == 0) return;
 
@@ -263,7 +280,7 @@ __global__ void __launch_bounds__(kLpRowThreads) logprob_rows_kernel(const LpArg
     cnt = __reduce_add_sync(0xffffffffu, cnt);
     if (lane == 0) {
       const bool ok = stat_valid(r);
-      const float log_s = ok ? logf(r.s) : NAN;
+      const float log_s = ok ? stat_log(r) : NAN;
       const int tok = token_id(a.tokens, row, a.V);
       const float xt = tok >= 0 ? (float)(static_cast<const T*>(a.logits) + row * a.ld)[tok] : NAN;
       o.logprob[row] = (xt - r.m) - log_s;

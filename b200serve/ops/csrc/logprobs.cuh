@@ -5,6 +5,8 @@
 // Slices join exactly: with M = max m_i and d_i = m_i - M,
 //   s = sum e^d_i s_i,   t = sum e^d_i (t_i + d_i s_i),
 //   log p(token) = (x_token - M) - log s,   entropy = log s - t / s.
+// Kept is r = s - 1, the sum without the largest logit's own term, and log s = log1p(r): beside an almost certain
+// token the others' small terms would lose their bits to the 1 (log p = -1e-4 would be off by 6e-4 of itself).
 // Everything is fp32. The terms of s lie in [0, 1] and those of t in [-1/e, 0]. An exponential carries ex2's 2^-22 and
 // the rounding of its argument d log2(e), 2^-23 |d| (|d| <= ln V where it matters), so log s is off by
 // about (1 + ln V) 2^-22; the sums, of at most 64 terms in a row and joined in trees, add a few 2^-24.
@@ -35,10 +37,10 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 struct RowStat {
-  float m, s, t;
+  float m, r, t;
 };
 
-// Adds slice (m, s, t) to `a`. m = -inf marks an empty slice (its s and t are 0). The differences are bounded so
+// Adds slice (m, r, t) to `a`. m = -inf marks an empty slice. The differences are bounded so
 // that a slice which does not count (all of it at the type's lowest value, say) adds e^d d s = 0, not 0 * -inf.
 __device__ __forceinline__ void stat_merge(RowStat& a, const RowStat& b) {
   const float M = fmaxf(a.m, b.m);
@@ -47,8 +49,8 @@ __device__ __forceinline__ void stat_merge(RowStat& a, const RowStat& b) {
     a = b;
   } else if (b.m != -INFINITY) {
     const float ea = __expf(da), eb = __expf(db);
-    a.t = ea * (a.t + da * a.s) + eb * (b.t + db * b.s);
-    a.s = ea * a.s + eb * b.s;
+    a.t = ea * (a.t + da * (1.f + a.r)) + eb * (b.t + db * (1.f + b.r));
+    a.r = ea * a.r + eb * b.r + fminf(ea, eb);           // the larger maximum's own term stays out
     a.m = M;
   }
 }
@@ -58,17 +60,18 @@ __device__ __forceinline__ RowStat stat_warp_merge(RowStat a) {
   for (int o = 16; o > 0; o >>= 1) {
     RowStat b;
     b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+    b.r = __shfl_xor_sync(0xffffffffu, a.r, o);
     b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
     stat_merge(a, b);
   }
   return a;
 }
 
-// A row has a distribution unless it holds a NaN or +inf (s is NaN then: +inf - +inf) or nothing
-// above -inf (s stays 0).
-__device__ __forceinline__ bool stat_valid(const RowStat& a) { return a.s > 0.f && a.m < INFINITY; }
+// A row has a distribution unless it holds a NaN or +inf (slices with a NaN are marked by m = +inf too) or nothing
+// above -inf.
+__device__ __forceinline__ bool stat_valid(const RowStat& a) { return a.m > -INFINITY && a.m < INFINITY; }
 
-__device__ __forceinline__ float stat_entropy(const RowStat& a) { return fmaxf(0.f, logf(a.s) - a.t / a.s); }
+__device__ __forceinline__ float stat_log(const RowStat& a) { return log1pf(a.r); }
+__device__ __forceinline__ float stat_entropy(const RowStat& a) { return fmaxf(0.f, log1pf(a.r) - a.t / (1.f + a.r)); }
 
 }  // namespace b200

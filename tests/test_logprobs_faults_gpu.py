@@ -90,3 +90,55 @@ def test_rows_that_overlap_in_memory():
         for x in (buf[:128].expand(T, -1), buf.as_strided((T, 128), (8, 1)), buf.as_strided((T, 128), (4, 1))):
             got, want = ops.linear_logprobs(x, w, tokens), ops.linear_logprobs(x.clone().contiguous(), w, tokens)
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# Log probabilities of almost certain tokens: -log1p(r), r = sum of the others' e^d. A term is off by ex2's (or, joining
+# slices, __expf's) 2^-21 and the rounding of d and d log2(e), 2^-23 |d| with |d| <= 40 here; the sums add 80 * 2^-24, log1p 2^-23:
+# 2^-21 + 40 * 2^-23 + 80 * 2^-24 + 2^-23 < 1.1e-5 of the value. Beside the 1 of a whole sum only 2^-24 = 6e-8 absolute is left.
+_CERTAIN = 1.1e-5
+
+
+def _certain_rows(V, n):
+    g = torch.Generator(device=dev).manual_seed(7)
+    x = torch.randn(n, V, device=dev, generator=g)
+    peak = torch.randint(0, V, (n,), device=dev, generator=g)
+    x[torch.arange(n, device=dev), peak] = torch.linspace(12, 38, n, device=dev)
+    return x, peak
+
+
+def _check_certain(lp, ent, logits, tokens):
+    d = logits.double() - logits.double().amax(-1, keepdim=True)
+    own = torch.zeros_like(d, dtype=torch.bool).scatter_(1, tokens[:, None], True)
+    e = d.exp().masked_fill(own, 0.0)
+    rest = e.sum(-1)
+    want = -torch.log1p(rest)
+    entropy = torch.log1p(rest) - (e * d).sum(-1) / (1 + rest)
+    assert float(want.abs().min()) < 1e-9 and float(want.abs().max()) > 0.02
+    assert float(((lp.double() - want) / want).abs().max()) < _CERTAIN
+    assert float(((ent.double() - entropy) / entropy).abs().max()) < 2 * _CERTAIN      # t carries the error of d as well
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [3000, 50001])
+def test_almost_certain_tokens(dtype, V):
+    x, peak = _certain_rows(V, 60)
+    x = x.to(dtype)
+    got = ops.token_logprobs(x, peak, top=2)
+    _check_certain(got.logprob, got.entropy, x, peak)
+    assert torch.equal(got.top_logprobs[:, 0], got.logprob) and torch.equal(got.top_ids[:, 0], peak.int())
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("T", [1, 60, 200])
+def test_almost_certain_tokens_of_the_head(packed, T):
+    """One-hot rows, so that the logits are the head's own bf16 numbers."""
+    V, H = 5000, 256
+    x, peak = _certain_rows(V, H)
+    w = x.t().contiguous().bfloat16()                                    # column h: the logits of the one-hot row h
+    rows = torch.linspace(0, H - 1, T, device=dev).long() if T > 1 else torch.tensor([H - 1], device=dev)
+    hot = torch.eye(H, device=dev).bfloat16()[rows]
+    lp, ent = ops.linear_logprobs(hot, ops.PackedWeight(w) if packed else w, peak[rows])
+    if T == 1:
+        assert -1e-9 < lp.item() < 0 and 0 < ent.item() < 1e-7
+    else:
+        _check_certain(lp, ent, w.float().t()[rows], peak[rows])
