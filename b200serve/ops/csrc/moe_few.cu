@@ -21,7 +21,7 @@
 // agree on), so a warp's load covers eight whole 64-byte pieces. The tensor pipe is a few percent
 // busy; tcgen05 tiles of 128 weight rows would only coarsen the units that balance the SMs. TMA
 // into shared memory was slower here: boxes of 8 rows and the waits on 24 stages took 0.25 us per
-// 8 KB and SM, 218 us where this takes 147 (16 rows, 128 experts of 768, top 8, 2048 wide).
+// 8 KB and SM, 218 us where this takes 148 (16 rows, 128 experts of 768, top 8, 2048 wide).
 //
 // Numerics: fp32 accumulation; the routing weight is folded into the activation in fp32, and the
 // activation is kept as the sum of two bf16 (high part and remainder, 16 bits of mantissa), so
