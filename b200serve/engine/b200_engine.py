@@ -476,7 +476,7 @@ class B200Engine(BaseEngine):
             if not r.done_event.wait(timeout):
                 raise TimeoutError("embedding request did not finish")
             if r.embedding is None:
-                raise RuntimeError("embedding failed: " + str(self._error or "engine error"))
+                raise RuntimeError("embedding failed: " + str(r.error or self._error or "engine error")) from r.error
         return [r.embedding for r in reqs], [len(r.tokens) for r in reqs]
 
     def score(self, prompts, timeout: float = 600.0):

@@ -19,6 +19,7 @@ that with in-replica continuous batching.
 from __future__ import annotations
 
 import itertools
+import logging
 import os
 import threading
 import time
@@ -31,6 +32,7 @@ from b200serve.engine.kv_cache import BLOCK, BlockAllocator
 from b200serve.engine.sampler import SamplingParams, sample
 from b200serve.ops import MAX_TOP_LOGPROBS
 
+_log = logging.getLogger(__name__)
 _ids = itertools.count()
 
 NGRAM_MAX, NGRAM_WINDOW = 3, 4096
@@ -77,7 +79,7 @@ class Request:
     embedding: list = None           # embedding requests: the mean-pooled final hidden state
     score: bool = False              # scoring requests (add_scoring): no generation
     scores: tuple = None             # their (log probabilities, entropies) of tokens[1:], nats
-    error: Exception = None          # why the scores could not be computed
+    error: Exception = None          # why the embedding or the scores could not be computed
     logprobs: list = field(default_factory=list)   # params.logprobs >= 0: one dict per output token
     mtp_draft: int = None            # MTP head's guess for the token after tokens[-1]
     mm: object = None                # models.qwen_vl.MMInput: images of a vision-language prompt
@@ -190,36 +192,50 @@ class Scheduler:
             seqs.append({"ids": list(r.tokens), "start": 0, "block_table": table, "hidden": True})
         if not seqs:
             return 0
+        results = {}
         try:
             hid = self.runner.prefill(seqs)
             off = 0
             for (r, table) in held:
-                n = len(r.tokens)
+                rows = hid[off:off + len(r.tokens)]
+                off += len(r.tokens)
                 if r.score:
-                    scores = ([], [])                # a single token has nothing to score
                     try:
-                        if n > 1:
-                            nxt = torch.as_tensor(r.tokens[1:], dtype=torch.long).to(hid.device)
-                            scores = tuple(t.tolist() for t in self.runner.score(hid[off:off + n - 1], nxt))
-                            self._check_layers()
-                            code = ops.linear_logprobs_error()
-                            if code:
-                                raise RuntimeError(f"a wait inside the scoring kernel ran out (code {code})")
-                        r.scores = scores            # None until then: how the caller tells a failed step
-                    except Exception as e:           # (no room, say) concerns this request alone
+                        results[id(r)] = self._score_rows(r, rows)
+                    except Exception as e:           # no room for it, say: the others go on
                         r.error = e
                 else:
-                    pooled = hid[off:off + n].float().mean(0).cpu().tolist()
-                    self._check_layers()
-                    r.embedding = pooled
-                off += n
-                r.state, r.finish_reason = "finished", "error" if r.error is not None else "stop"
-                r.finish_time = time.perf_counter()
+                    results[id(r)] = rows.float().mean(0).cpu().tolist()
+            self._check_layers()                     # before any of the step's results is handed out
+        except Exception as e:                       # nor does it end the generations under way
+            _log.exception("embedding step failed")
+            results = {}
+            for r, _ in held:
+                r.error = r.error or e
         finally:
             for r, table in held:
+                if id(r) in results:
+                    if r.score:
+                        r.scores = results[id(r)]
+                    else:
+                        r.embedding = results[id(r)]
+                r.state, r.finish_reason = "finished", "stop" if id(r) in results else "error"
+                r.finish_time = time.perf_counter()
                 self.alloc.release(table)
                 r.done_event.set()
         return 0
+
+    def _score_rows(self, r: Request, hid) -> tuple:
+        """(log probabilities, entropies) of tokens[1:] from the request's final-normed hidden rows."""
+        n = len(r.tokens)
+        if n == 1:                                   # nothing to score
+            return [], []
+        nxt = torch.as_tensor(r.tokens[1:], dtype=torch.long).to(hid.device)
+        scores = tuple(t.tolist() for t in self.runner.score(hid[:n - 1], nxt))
+        code = ops.linear_logprobs_error()
+        if code:
+            raise RuntimeError(f"a wait inside the scoring kernel ran out (code {code})")
+        return scores
 
     def metrics(self) -> dict:
         return {**self.stats, "running": len(self.running), "waiting": len(self.waiting),

@@ -167,3 +167,52 @@ def test_a_worker_rank_stops_after_a_layer_gave_up(monkeypatch):
     runner = SimpleNamespace(device="cpu", pipeline_step=lambda slot: None)
     with pytest.raises(RuntimeError, match="code 24"):
         worker.worker_loop(runner, comm)
+
+
+def _with_generation(engine, start):
+    """``start()`` while a generation is under way, which has to end as it would alone; what start() raised or returned."""
+    from b200serve.engine.scheduler import Request
+    prompt, params = list(range(10, 30)), SamplingParams(max_tokens=40, ignore_eos=True)
+    [want] = engine.generate([prompt], params, timeout=60)
+    req = engine.submit(Request(prompt=prompt, params=params))
+    try:
+        out = start()
+    except RuntimeError as e:
+        out = e
+    assert req.done_event.wait(60) and req.finish_reason == "length" and req.output == want.output
+    return out
+
+
+def test_a_failed_embedding_step_leaves_generations_alone(engine, monkeypatch):
+    real = engine.runner.prefill
+
+    def prefill(seqs):
+        if any(s.get("hidden") for s in seqs):
+            raise MemoryError("no room for the activations")
+        return real(seqs)
+
+    monkeypatch.setattr(engine.runner, "prefill", prefill)
+    free = engine.scheduler.alloc.num_free
+    for call in (lambda: engine.score([[1, 2, 3], [4, 5]], timeout=60), lambda: engine.embed(["some text"], timeout=60)):
+        out = _with_generation(engine, call)
+        assert isinstance(out, RuntimeError) and "no room for the activations" in str(out)
+    monkeypatch.undo()
+    assert engine.scheduler.alloc.num_free == free and len(engine.score([[1, 2, 3]], timeout=60)[0]["logprobs"]) == 2
+
+
+def test_a_void_step_fails_all_of_its_inputs(engine, monkeypatch):
+    """One prefill, one error word: the first input that reads it must not clear it for the others."""
+    from b200serve import ops
+    from b200serve.engine.scheduler import Request
+    codes = []
+    monkeypatch.setattr(ops, "moe_layer_error", lambda reset=True, wait=True: codes.pop() if codes else 0)
+    params = SamplingParams(max_tokens=1)
+    reqs = [Request(prompt=p, params=params) for p in ([1, 2, 3], [4, 5, 6], [7, 8])]
+    engine.stop_loop()                                       # the three of them in one step
+    for r in reqs[:2]:
+        engine.scheduler.add_scoring(r)
+    engine.scheduler.add_embedding(reqs[2])
+    codes.append(24)
+    engine.scheduler._embed_step()
+    assert all(r.done_event.is_set() and "code 24" in str(r.error) and r.finish_reason == "error" for r in reqs)
+    assert all(r.scores is None and r.embedding is None for r in reqs)
