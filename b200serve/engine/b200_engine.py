@@ -500,6 +500,7 @@ class B200Engine(BaseEngine):
             self._wake.notify_all()
         for r in reqs:
             if not r.done_event.wait(timeout):
+                self.scheduler.drop_embedding(reqs)
                 raise TimeoutError("scoring request did not finish")
             if r.scores is None:
                 raise RuntimeError("scoring failed: " + str(r.error or self._error or "engine error")) from r.error

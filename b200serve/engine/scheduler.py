@@ -159,6 +159,12 @@ class Scheduler:
             self.embed_waiting.append(req)
         return req
 
+    def drop_embedding(self, reqs):
+        """Take those of ``reqs`` (embedding or scoring inputs) that no step has begun out of the queue."""
+        gone = {id(r) for r in reqs}
+        with self.lock:
+            self.embed_waiting[:] = [r for r in self.embed_waiting if id(r) not in gone]
+
     def add_scoring(self, req: Request) -> Request:
         """Queue a token sequence whose tokens' log probabilities are wanted (no generation)."""
         req.score = True

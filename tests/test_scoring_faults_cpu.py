@@ -216,3 +216,13 @@ def test_a_void_step_fails_all_of_its_inputs(engine, monkeypatch):
     engine.scheduler._embed_step()
     assert all(r.done_event.is_set() and "code 24" in str(r.error) and r.finish_reason == "error" for r in reqs)
     assert all(r.scores is None and r.embedding is None for r in reqs)
+
+
+def test_a_call_that_timed_out_leaves_nothing_queued(engine, monkeypatch):
+    monkeypatch.setattr(engine.scheduler, "step", lambda: 0)             # a step that takes for ever
+    monkeypatch.setattr(engine.scheduler, "has_work", lambda: False)
+    with pytest.raises(TimeoutError):
+        engine.score([[1, 2, 3], [4, 5, 6]], timeout=0.2)
+    assert engine.scheduler.embed_waiting == []
+    monkeypatch.undo()
+    assert len(engine.score([[1, 2, 3]], timeout=60)[0]["logprobs"]) == 2
