@@ -7,7 +7,7 @@
 //   thread of the epilogue owns a row and sums up a slice's maximum and exponential sums in
 //   registers, with no exchange between threads. Per (row, 128 columns) 16 bytes are written
 //   instead of 512 of logits.
-//   linear_logprob_rows: joins the slices of every row.
+//   linear_logprob_rows: joins the slices of every row, with the token's own logit computed once more.
 //
 // With more than 128 rows two CTAs of a cluster work on one tile of 256 rows (cta_group::2): each
 // loads its 128 rows of x and half of the tile's columns of w, so an SM reads 32 KB for 64 elements of H
@@ -62,6 +62,10 @@ struct LlArgs {
   float softcap, inv_softcap;
   TokenIds tokens;
   int per_tile;                          // slices of up to 128 columns in a tile: 1 or 2
+  int H;
+  const __nv_bfloat16* x;                // [T, H], row stride ldx; with w the token's own logit is computed again
+  const __nv_bfloat16* w;
+  long long ldx;
   float4* part;                          // [v_tiles * per_tile][T] (m, r, t, the token's logit where the slice has it)
 };
 
@@ -380,18 +384,59 @@ __global__ void __launch_bounds__(kLlThreads, 1)
   }
 }
 
+// This thread's share (one of G) of the product of row `row` of x with the token's row of w, rounded to nearest.
+template <int G>
+__device__ __forceinline__ float ll_token_dot(const LlArgs& a, int row, int tok, int g) {
+  const __nv_bfloat16* x = a.x + row * a.ldx;
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i] = 0.f;
+  constexpr int U = 4;                                 // pieces on the way at a time
+  for (int k0 = g * 8; k0 < a.H; k0 += U * G * 8) {
+    bf16x8 xv[U], wv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * G * 8;
+      xv[u] = wv[u] = bf16x8{};
+      if (k < a.H) {
+        xv[u] = *reinterpret_cast<const bf16x8*>(x + k);
+        wv[u] = *reinterpret_cast<const bf16x8*>(
+            a.packed ? a.w + (((size_t)(tok >> 7) * a.kb_total + (k >> 6)) * 128 + (tok & 127)) * 64 + (k & 63)
+                     : a.w + (size_t)tok * a.H + k);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float xf[8], wf[8];
+      unpack8(xv[u], xf);
+      unpack8(wv[u], wf);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = fmaf(xf[i], wf[i], s[i]);
+    }
+  }
+  return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+}
+
 // 256 threads per CTA on R rows, neighbouring threads on neighbouring rows. A thread takes its slices eight at
 // a time: one maximum for the eight and the running sum, so the chain of rescalings is short.
+//
+// The token's own logit is computed once more, by rounded additions in a tree, and takes the place of the tensor cores'
+// one in the statistics: where the token is likely, its products are mostly positive, all cuts go the same way (a logit of 13
+// is off by 1.7e-6 with parts of 128 elements, by 6.6e-6 with 512) and every bit of log p hangs on that logit. It
+// takes 9 of the 2000 us of 2048 rows of H = 4096, and 2 of the 200 of one row.
 constexpr int kLlRowThreads = 256;
 template <int R>
 __global__ void __launch_bounds__(kLlRowThreads) linear_logprob_rows_kernel(const LlArgs a, float* __restrict__ logprob,
                                                                             float* __restrict__ entropy) {
   constexpr int G = kLlRowThreads / R;                 // threads per row
   __shared__ RowStat st[G][R];
+  __shared__ float dots[G][R];
   pdl_wait();
   pdl_trigger();
   const int r = threadIdx.x % R, g = threadIdx.x / R;
   const int row = blockIdx.x * R + r, S = a.v_tiles * a.per_tile;
+  const int tok = row < a.T ? token_id(a.tokens, row, a.V) : -1;
+  float dot = tok >= 0 ? ll_token_dot<G>(a, row, tok, g) : 0.f;
   RowStat acc{-INFINITY, 0.f, 0.f};
   if (row < a.T) {
     for (int i0 = g; i0 < S; i0 += 8 * G) {
@@ -421,22 +466,38 @@ __global__ void __launch_bounds__(kLlRowThreads) linear_logprob_rows_kernel(cons
     }
   }
   st[g][r] = acc;
+  dots[g][r] = dot;
   __syncthreads();
 #pragma unroll
   for (int o = G / 2; o > 0; o >>= 1) {
     if (g < o) {
       stat_merge(acc, st[g + o][r]);
       st[g][r] = acc;
+      dots[g][r] = dot += dots[g + o][r];
     }
     __syncthreads();
   }
   if (g != 0 || row >= a.T) return;
   const bool ok = stat_valid(acc) && __ldcg(&g_ll_err) == 0;
-  const int tok = token_id(a.tokens, row, a.V);
   float xt = NAN;
   if (tok >= 0) {
     const int v_tile = tok / a.tile_n, half = (tok - v_tile * a.tile_n) / kLlCols;
     xt = __ldcg(&a.part[(size_t)(v_tile * a.per_tile + half) * a.T + row].w);
+    if (a.softcap > 0.f) dot = a.softcap * tanhf(dot * a.inv_softcap);
+    const float delta = dot - xt;                      // not finite where the logit is not: the first one stays then
+    if (fabsf(delta) <= 1.f) {
+      if (xt == acc.m) {                               // the token leads: all others move by -delta
+        const float q = expm1f(-delta);
+        acc.t = (1.f + q) * (acc.t - delta * acc.r);
+        acc.r += q * acc.r;
+        acc.m = dot;
+      } else {
+        const float p = __expf(xt - acc.m), q = expm1f(delta);
+        acc.t += p * ((1.f + q) * (dot - acc.m) - (xt - acc.m));
+        acc.r += p * q;
+      }
+      xt = dot;
+    }
   }
   logprob[row] = ok ? (xt - acc.m) - stat_log(acc) : NAN;
   entropy[row] = ok ? stat_entropy(acc) : NAN;
@@ -503,9 +564,9 @@ std::vector<torch::Tensor> linear_logprobs(torch::Tensor x, torch::Tensor w, int
     const int64_t slices = (int64_t)a.v_tiles * a.per_tile;
     a.inv_softcap = softcap > 0.0 ? (float)(1.0 / softcap) : 0.f;
     // 128 elements per part where the read of w is the bound, else 512 (the epilogue's additions then stay under the
-    // MMAs: 2048 rows of H = 4096 take 2.00 ms, parts of 256 2.18). Root-mean-square error of a log probability, logits
-    // up to 15: 6.2e-7 for 128, 9.0e-7 for 256, 1.8e-6 for 512 elements (a rounded fp32 product 3.8e-6, one row of it
-    // 3.7e-7); below 128 the roundings of the many additions take over. One row of 151936 x 4096: 201 us,
+    // MMAs: 2048 rows of H = 4096 take 2.00 ms, parts of 256 2.18). Root-mean-square error of a log probability beside
+    // the logits', H = 4096: 3.6e-7 for 128, 5.4e-7 for 256, 1.1e-6 for 512 elements, before the token's own logit
+    // is computed again; below 128 the roundings of the many additions take over. One row of 151936 x 4096: 201 us,
     // with parts of 256 195, of 64 228.
     a.part_kb = cg == 1 ? 2 : 8;
     a.softcap = (float)softcap;
@@ -514,7 +575,8 @@ std::vector<torch::Tensor> linear_logprobs(torch::Tensor x, torch::Tensor w, int
     const int64_t need = slices * a.T * 4;
     if (!part.defined() || part.numel() < need) part = torch::empty({need}, logprob.options());
     a.part = reinterpret_cast<float4*>(part.data_ptr());
-    const void* xp = static_cast<const __nv_bfloat16*>(x.data_ptr()) + t0 * ldx;
+    const __nv_bfloat16* xp = static_cast<const __nv_bfloat16*>(x.data_ptr()) + t0 * ldx;
+    a.H = (int)H; a.x = xp; a.w = static_cast<const __nv_bfloat16*>(w.data_ptr()); a.ldx = ldx;
     const uint64_t xd[2] = {(uint64_t)H, (uint64_t)a.T}, xs[1] = {(uint64_t)ldx * 2};
     a.x_rows = cg == 2 ? kLlBM : (a.T + 15) / 16 * 16;
     a.stage_bytes = (a.x_rows + a.tile_n / cg) * 128;

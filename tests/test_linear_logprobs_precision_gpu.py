@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from b200serve import ops
-from logprob_cases import check_linear_logprobs
+from logprob_cases import INF, check_linear_logprobs
 
 pytestmark = pytest.mark.gpu
 dev = "cuda"
@@ -96,3 +96,30 @@ def test_few_rows_are_as_exact_as_a_rounded_product():
     assert err.pow(2).mean().sqrt().item() < 4.8e-7 * rms
     lp, _ = ops.linear_logprobs(x, w, tokens)
     assert (lp.double() - want).pow(2).mean().sqrt().item() < 4.8e-7 * rms
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("T", [1, 40, 200, 1000])
+def test_likely_tokens(packed, T):
+    """Rows that lean towards their token: the products of its logit (4 to 16) are mostly positive, so that cuts would all
+    go one way. log p = -log1p(r), r = sum e^(x_j - x_token) over thousands of small terms whose own errors cancel; what
+    moves all of them is the token's logit: half a last place of it (below 16) 4.8e-7, its sum of 8-element chains and a
+    tree a third of that (1.6e-7, independent), and ex2's bias, at most 2^-22 = 2.4e-7: 7.5e-7 of log p. Left out:
+    rows with another leader (log p is a difference of logits then, with that one's error) and logits from 16 on."""
+    V, H = 6000, 4096
+    w = (torch.randn(V, H, device=dev) * 1.3 / math.sqrt(H)).bfloat16()
+    tokens = torch.randint(0, V, (T,), device=dev)
+    lift = torch.linspace(11.5, 15, T, device=dev)[:, None] / 1.69
+    x = (torch.randn(T, H, device=dev) * 0.5 + lift * w[tokens].float()).bfloat16()
+    z = x.double() @ w.double().t()
+    top = z.gather(1, tokens[:, None])[:, 0]
+    d = (z - top[:, None]).scatter_(1, tokens[:, None], -INF)
+    rest = d.exp().sum(-1)
+    lead = (d.amax(-1) < 0) & (top < 16)
+    want, ent = -torch.log1p(rest), torch.log1p(rest) - (d.exp() * d.clamp_min(-1e30)).sum(-1) / (1 + rest)
+    lp, en = ops.linear_logprobs(x, ops.PackedWeight(w) if packed else w, tokens)
+    rel = ((lp.double() - want) / want)[lead]
+    assert float(lead.float().mean()) > 0.9
+    assert rel.pow(2).mean().sqrt().item() < 7.5e-7
+    # the entropy's terms carry d e^d: twice as much
+    assert (((en.double() - ent) / ent)[lead]).pow(2).mean().sqrt().item() < 1.5e-6
